@@ -2,7 +2,8 @@
 
 ``hyperflow_h3_flash_b200.int8`` mirrors ``hyperflow_h3_flash.int8`` (src/hyperflow_h3_flash/int8.py);
 ``hyperflow_h3_flash_b200.ulysses`` shards token rows over GPUs with the seq<->head all-to-all around attention;
-``libconvrot.so`` (C ABI: include/convrot.h) holds the CUDA kernels.
+``hyperflow_h3_flash_b200.attention`` holds what an attention block computes between those linears (rotary table, per-head
+q / k norm with rotation, packed attention); ``libconvrot.so`` (C ABI: include/convrot.h) holds the CUDA kernels.
 """
 
 from .int8 import (

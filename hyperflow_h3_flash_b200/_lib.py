@@ -45,6 +45,12 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "convrot_peer_signal": ([_P, _I, _U32, _P], _I),
     "convrot_peer_wait": ([_P, _I, _U32, _P], _I),
     "convrot_copy_blocks": ([_P, _P, _P, _I, _P], _I),
+    "convrot_rotary_table": ([_P, _I, _L, _L, _I, _P, _P, _P, _P], _I),
+    "convrot_qk_norm_rope": ([_P, _L, _L, _P, _L, _L, _I, _P, _L, _L, _P, _L, _L, _I, _L, _I, _I, _I, _P, _P, _I,
+                              ctypes.c_float, _P, _L, _I, _I, _P], _I),
+    "convrot_attention_workspace_size": ([_L, _L, _L, _I, _I, _I], _L),
+    "convrot_attention": ([_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _L, _L, _L, _I, _I, _I, _I, ctypes.c_float, _I,
+                           _P, _L, _L, _P, _P, _S, _P], _I),
     "convrot_workspace_size": ([_L, _L, _L], _S),
     "convrot_linear": ([_P, _L, _P, _L, _P, _P, _P, _L, _P, _L, _L, _L, _L, _L, _I, _P, _S, _P, _L, _P], _I),
     "convrot_linear_noalloc": ([_P, _L, _P, _L, _P, _P, _P, _L, _P, _L, _L, _L, _L, _L, _I, _P, _L, _P], _I),

@@ -1,0 +1,258 @@
+// Host side of the attention operators (argument checks, tensor maps, launch shapes); included by convrot.cu inside its
+// unnamed namespace, after the device state and tensor-map helpers.  Contracts: include/convrot.h.
+
+// ------------------------------------------------------------------------------------------------ rotary table
+
+int rotary_table(const void* pos, int pos_type, int64_t ld_pos, int64_t rows, int axes, const int* dims,
+                 const double* theta, float* out, cudaStream_t stream) {
+  if (axes < 1 || axes > kRopeMaxAxes) return CONVROT_ERR_SHAPE;
+  if (!dims || !theta || pos_type < 0 || pos_type > 3) return CONVROT_ERR_ARG;
+  RotaryTableParams p;
+  memset(&p, 0, sizeof(p));
+  for (int a = 0; a < axes; ++a) {
+    if (dims[a] <= 0 || dims[a] % 2 || p.pairs + dims[a] / 2 > kRopeMaxPairs) return CONVROT_ERR_SHAPE;
+    if (!(theta[a] > 0.0) || !isfinite(theta[a])) return CONVROT_ERR_ARG;
+    for (int i = 0; i < dims[a] / 2; ++i, ++p.pairs) {
+      p.freq_over_pi[p.pairs] = pow(theta[a], -2.0 * i / dims[a]) / 3.14159265358979323846;
+      p.axis[p.pairs] = static_cast<uint8_t>(a);
+    }
+  }
+  if (rows < 0 || rows > INT32_MAX || ld_pos < axes) return CONVROT_ERR_SHAPE;
+  if (rows == 0) return CONVROT_OK;
+  if (!pos || !out) return CONVROT_ERR_ARG;
+  const int size = pos_type == 1 || pos_type == 3 ? 8 : 4;
+  if (reinterpret_cast<uintptr_t>(pos) % size || !aligned16(out)) return CONVROT_ERR_ALIGN;
+  DeviceState* st = nullptr;
+  int rc = device_state(&st);
+  if (rc) return rc;
+  p.pos = pos;
+  p.ld_pos = ld_pos;
+  p.rows = rows;
+  p.out = reinterpret_cast<float2*>(out);
+  const int64_t need = (rows * p.pairs + 255) / 256, most = 16 * static_cast<int64_t>(st->sms);
+  const unsigned grid = static_cast<unsigned>(need < most ? need : most);
+  switch (pos_type) {
+    case 0: rotary_table_kernel<int32_t><<<grid, 256, 0, stream>>>(p); break;
+    case 1: rotary_table_kernel<int64_t><<<grid, 256, 0, stream>>>(p); break;
+    case 2: rotary_table_kernel<float><<<grid, 256, 0, stream>>>(p); break;
+    default: rotary_table_kernel<double><<<grid, 256, 0, stream>>>(p); break;
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? CONVROT_OK : cuda_fail(e);
+}
+
+// ------------------------------------------------------------------------------------------------ norm and rotation
+
+int qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h, int heads_q,
+                 const void* k, int64_t k_t, int64_t k_h, void* k_out, int64_t ko_t, int64_t ko_h, int heads_k,
+                 int64_t rows, int D, int dtype, int norm, const void* q_weight, const void* k_weight, int weight_f32,
+                 float eps, const float* table, int64_t ld_table, int R, int interleaved, cudaStream_t stream) {
+  if (dtype < 0 || dtype > 1) return CONVROT_ERR_ARG;
+  if (D < 8 || D > 256 || D % 8 || heads_q < 1 || heads_k < 0 || heads_q > (1 << 20) || heads_k > (1 << 20) ||
+      rows < 0 || rows > INT32_MAX)
+    return CONVROT_ERR_SHAPE;
+  if (!norm && !table) return CONVROT_ERR_ARG;
+  if (!norm && (q_weight || k_weight)) return CONVROT_ERR_ARG;
+  if (norm && !(eps >= 0.0f && eps < 3e38f)) return CONVROT_ERR_ARG;
+  if (table) {
+    if (R < 8 || R > D || R % (interleaved ? 8 : 16) || ld_table < R / 2) return CONVROT_ERR_SHAPE;
+    if (ld_table % 2 || !aligned16(table)) return CONVROT_ERR_ALIGN;
+  }
+  if (rows == 0) return CONVROT_OK;
+  if (!q || !q_out || (heads_k > 0 && (!k || !k_out))) return CONVROT_ERR_ARG;
+  const int64_t strides[] = {q_t, q_h, qo_t, qo_h, k_t, k_h, ko_t, ko_h};
+  for (int i = 0; i < (heads_k ? 8 : 4); ++i) {
+    if (strides[i] < 0) return CONVROT_ERR_SHAPE;
+    if (strides[i] % 8) return CONVROT_ERR_ALIGN;
+  }
+  if (!aligned16(q) || !aligned16(q_out) || !aligned16(k) || !aligned16(k_out) || !aligned16(q_weight) ||
+      !aligned16(k_weight))
+    return CONVROT_ERR_ALIGN;
+  DeviceState* st = nullptr;
+  int rc = device_state(&st);
+  if (rc) return rc;
+  QkRopeParams p;
+  memset(&p, 0, sizeof(p));
+  p.in[0] = q, p.in[1] = k;
+  p.out[0] = q_out, p.out[1] = k_out;
+  p.in_t[0] = q_t, p.in_h[0] = q_h, p.out_t[0] = qo_t, p.out_h[0] = qo_h;
+  p.in_t[1] = k_t, p.in_h[1] = k_h, p.out_t[1] = ko_t, p.out_h[1] = ko_h;
+  p.weight[0] = q_weight, p.weight[1] = k_weight;
+  p.heads[0] = heads_q, p.heads[1] = heads_k;
+  p.table = reinterpret_cast<const float2*>(table);
+  p.ld_table = ld_table;
+  p.rows = rows;
+  p.D = D;
+  p.R = table ? R : 0;
+  while ((8 << p.lanes_log2) < D) ++p.lanes_log2;
+  const int per = kRopeRows * (32 >> p.lanes_log2);
+  p.items = (heads_q + heads_k + per - 1) / per;
+  p.norm = norm;
+  p.weight_f32 = weight_f32;
+  p.eps = eps;
+  const int64_t blocks = (rows * p.items + kRopeWarps - 1) / kRopeWarps;
+  if (blocks > INT32_MAX) return CONVROT_ERR_SHAPE;
+  const unsigned grid = static_cast<unsigned>(blocks);
+  const int threads = kRopeWarps * 32;
+  if (dtype == 0) {
+    if (interleaved)
+      qk_norm_rope_kernel<__nv_bfloat16, true><<<grid, threads, 0, stream>>>(p);
+    else
+      qk_norm_rope_kernel<__nv_bfloat16, false><<<grid, threads, 0, stream>>>(p);
+  } else {
+    if (interleaved)
+      qk_norm_rope_kernel<__half, true><<<grid, threads, 0, stream>>>(p);
+    else
+      qk_norm_rope_kernel<__half, false><<<grid, threads, 0, stream>>>(p);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? CONVROT_OK : cuda_fail(e);
+}
+
+// ------------------------------------------------------------------------------------------------ attention
+
+int attn_check(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int D) {
+  if (Tq < 0 || Tk < 0 || Tq > INT32_MAX / 2 || Tk > INT32_MAX / 2 || batch < 0 || batch > (1 << 20))
+    return CONVROT_ERR_SHAPE;
+  if (heads_kv < 1 || heads_q < 1 || heads_q % heads_kv || heads_q / heads_kv > kAtTile || heads_q > (1 << 16))
+    return CONVROT_ERR_SHAPE;
+  if (D < 8 || D > 128 || D % 8) return CONVROT_ERR_SHAPE;
+  return CONVROT_OK;
+}
+
+// How keys are split, from host-known sizes alone.
+void attn_plan(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int D, int sms, int* max_splits,
+               int* chunk_tiles) {
+  *max_splits = 1;
+  *chunk_tiles = 1;
+  if (batch < 1 || Tq < 1 || Tk < 1) return;
+  const int64_t positions = kAtTile / (heads_q / heads_kv);
+  const int64_t span = 2 * positions;
+  const int64_t q_tiles = batch > (Tq + span - 1) / span ? batch : (Tq + span - 1) / span;
+  const int64_t items = q_tiles * heads_kv;
+  const int64_t k_tiles = (Tk + kAtTile - 1) / kAtTile;  // of all sequences; one may hold them all
+  const int64_t mean = (k_tiles + batch - 1) / batch;
+  if (items >= 3 * sms && Tq > 4 * batch) return;
+  int64_t chunk = (items * mean + 4 * sms - 1) / (4 * sms);
+  if (chunk < 4) chunk = 4;
+  int64_t splits = (k_tiles + chunk - 1) / chunk;
+  const int64_t bytes = Tq * heads_q * (D + 1) * 4;
+  const int64_t most = (int64_t{96} << 20) / bytes;
+  if (splits > most) splits = most;
+  if (splits > 64) splits = 64;
+  if (splits <= 1) return;
+  *max_splits = static_cast<int>(splits);
+  *chunk_tiles = static_cast<int>(chunk);
+}
+
+int attn_map(CUtensorMap* map, const void* base, int dtype, int D, int64_t heads, int64_t rows, int64_t ld_h,
+             int64_t ld_t, int box_heads, int box_rows) {
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld_h * 2), static_cast<cuuint64_t>(ld_t * 2)};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    t_last_cuda_error = static_cast<int>(r);
+    return CONVROT_ERR_CUDA;
+  }
+  return CONVROT_OK;
+}
+
+template <class T, int NP>
+int launch_attention(const DeviceState& st, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                     const AttnParams& p, int64_t items, cudaStream_t stream) {
+  auto kernel = attention_kernel<T, NP>;
+  int ready = -1;
+  int rc = cached_resident(reinterpret_cast<const void*>(kernel), &ready);
+  if (rc) return rc;
+  cudaError_t e;
+  if (ready < 0) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, AttnCfg<NP>::kSmemBytes);
+    if (e != cudaSuccess) return cuda_fail(e);
+    store_resident(reinterpret_cast<const void*>(kernel), 1);
+  }
+  const unsigned grid = static_cast<unsigned>(items < st.sms ? items : st.sms);
+  kernel<<<grid, kAtThreads, AttnCfg<NP>::kSmemBytes, stream>>>(tq, tk, tv, p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e);
+  if (p.max_splits > 1) {
+    const int64_t rows = static_cast<int64_t>(p.Tq) * p.heads_kv * p.group;
+    attention_combine_kernel<T><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e);
+  }
+  return CONVROT_OK;
+}
+
+int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v,
+              int64_t v_t, int64_t v_h, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t Tq, int64_t Tk,
+              int heads_q, int heads_kv, int D, int dtype, float scale, int causal, void* out, int64_t out_t,
+              int64_t out_h, float* lse, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  int rc = attn_check(Tq, Tk, batch, heads_q, heads_kv, D);
+  if (rc) return rc;
+  if (dtype < 0 || dtype > 1 || !(scale > 0.0f) || !(scale < 3e38f)) return CONVROT_ERR_ARG;
+  if ((cu_q == nullptr) != (cu_k == nullptr) || (!cu_q && batch != 1)) return CONVROT_ERR_ARG;
+  if (Tq == 0 || batch == 0) return CONVROT_OK;
+  if (!q || !out || (Tk > 0 && (!k || !v))) return CONVROT_ERR_ARG;
+  const struct {
+    const void* base;
+    int64_t t, h, heads, rows;
+  } ops[4] = {{q, q_t, q_h, heads_q, Tq}, {out, out_t, out_h, heads_q, Tq}, {k, k_t, k_h, heads_kv, Tk},
+              {v, v_t, v_h, heads_kv, Tk}};
+  for (int i = 0; i < 4; ++i) {
+    if (!aligned16(ops[i].base) || ops[i].t % 8 || ops[i].h % 8) return CONVROT_ERR_ALIGN;
+    if (ops[i].t <= 0 || ops[i].h <= 0 || ops[i].t >= (int64_t{1} << 38) || ops[i].h >= (int64_t{1} << 38))
+      return CONVROT_ERR_SHAPE;
+  }
+  if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k) | reinterpret_cast<uintptr_t>(lse)) & 3u)
+    return CONVROT_ERR_ALIGN;
+  DeviceState* st = nullptr;
+  if ((rc = device_state(&st))) return rc;
+  AttnParams p;
+  memset(&p, 0, sizeof(p));
+  attn_plan(Tq, Tk, batch, heads_q, heads_kv, D, st->sms, &p.max_splits, &p.chunk_tiles);
+  if (p.max_splits > 1) {
+    const size_t rows = static_cast<size_t>(p.max_splits) * Tq * heads_q;
+    if (!workspace || workspace_bytes < rows * (D + 1) * 4) return CONVROT_ERR_ARG;
+    if (!aligned16(workspace)) return CONVROT_ERR_ALIGN;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_lse = p.part_o + rows * D;
+  }
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.batch = static_cast<int>(batch);
+  p.Tq = static_cast<int>(Tq);
+  p.Tk = static_cast<int>(Tk);
+  p.heads_kv = heads_kv;
+  p.group = heads_q / heads_kv;
+  p.D = D;
+  p.positions = kAtTile / p.group;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.causal = causal ? 1 : 0;
+  p.out = out;
+  p.out_t = out_t;
+  p.out_h = out_h;
+  p.lse = lse;
+  p.wait_limit_ns = g_wait_limit_ns;
+  p.error_word = st->error_word;
+  CUtensorMap tq, tk, tv;
+  if ((rc = attn_map(&tq, q, dtype, D, heads_q, Tq, q_h, q_t, p.group, p.positions))) return rc;
+  // Without a key the maps of k and v are never read; the query's stands in (an empty extent cannot be encoded).
+  if ((rc = attn_map(&tk, Tk ? k : q, dtype, D, Tk ? heads_kv : heads_q, Tk ? Tk : Tq, Tk ? k_h : q_h, Tk ? k_t : q_t, 1,
+                     kAtTile)))
+    return rc;
+  if ((rc = attn_map(&tv, Tk ? v : q, dtype, D, Tk ? heads_kv : heads_q, Tk ? Tk : Tq, Tk ? v_h : q_h, Tk ? v_t : q_t, 1,
+                     kAtTile)))
+    return rc;
+  // An upper bound of the work items (the kernel finds their number): every CTA beyond it would find nothing.
+  const int64_t span = 2 * p.positions;
+  const int64_t q_tiles = batch == 1 ? (Tq + span - 1) / span : Tq / span + (batch < Tq ? batch : Tq);
+  const int64_t items = q_tiles * heads_kv * p.max_splits;
+  if (dtype == 0)
+    return D <= 64 ? launch_attention<__nv_bfloat16, 1>(*st, tq, tk, tv, p, items, stream)
+                   : launch_attention<__nv_bfloat16, 2>(*st, tq, tk, tv, p, items, stream);
+  return D <= 64 ? launch_attention<__half, 1>(*st, tq, tk, tv, p, items, stream)
+                 : launch_attention<__half, 2>(*st, tq, tk, tv, p, items, stream);
+}

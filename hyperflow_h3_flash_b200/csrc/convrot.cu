@@ -7,6 +7,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -14,9 +15,11 @@
 #include <mutex>
 
 #include "../../include/convrot.h"
+#include "attention.cuh"
 #include "gemm_sm100.cuh"
 #include "gemm_sm100_2sm.cuh"
 #include "peer.cuh"
+#include "qk_rope.cuh"
 #include "rotate_quant.cuh"
 
 namespace convrot {
@@ -752,6 +755,8 @@ int noalloc_scratch(uint8_t** out) {
   return CONVROT_OK;
 }
 
+#include "attention_api.cuh"
+
 }  // namespace
 }  // namespace convrot
 
@@ -1012,6 +1017,40 @@ int convrot_linear_noalloc(const void* x, int64_t ldx, const int8_t* w, int64_t 
   // part of the scratch completely before anything reads it, so no part needs clearing between calls.
   return convrot_linear(x, ldx, w, ldw, ws, bias, lr_down, ld_down, lr_up, ld_up, r, M, N, K, group, scratch,
                         CONVROT_NOALLOC_SCRATCH_BYTES, y, ldy, stream);
+}
+
+int convrot_rotary_table(const void* positions, int pos_type, int64_t ld_pos, int64_t rows, int axes, const int* dims,
+                         const double* theta, float* out, void* stream) {
+  return rotary_table(positions, pos_type, ld_pos, rows, axes, dims, theta, out, static_cast<cudaStream_t>(stream));
+}
+
+int convrot_qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h, int heads_q,
+                         const void* k, int64_t k_t, int64_t k_h, void* k_out, int64_t ko_t, int64_t ko_h, int heads_k,
+                         int64_t rows, int D, int dtype, int norm, const void* q_weight, const void* k_weight,
+                         int weight_f32, float eps, const float* table, int64_t ld_table, int R, int interleaved,
+                         void* stream) {
+  return qk_norm_rope(q, q_t, q_h, q_out, qo_t, qo_h, heads_q, k, k_t, k_h, k_out, ko_t, ko_h, heads_k, rows, D, dtype,
+                      norm, q_weight, k_weight, weight_f32, eps, table, ld_table, R, interleaved,
+                      static_cast<cudaStream_t>(stream));
+}
+
+int64_t convrot_attention_workspace_size(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int D) {
+  if (attn_check(Tq, Tk, batch, heads_q, heads_kv, D)) return -1;
+  if (Tq == 0 || batch == 0) return 0;
+  DeviceState* st = nullptr;
+  if (device_state(&st)) return -1;
+  int splits = 1, chunk = 1;
+  attn_plan(Tq, Tk, batch, heads_q, heads_kv, D, st->sms, &splits, &chunk);
+  return splits > 1 ? splits * Tq * heads_q * (D + 1) * 4 : 0;
+}
+
+int convrot_attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v,
+                      int64_t v_t, int64_t v_h, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t Tq,
+                      int64_t Tk, int heads_q, int heads_kv, int D, int dtype, float scale, int causal, void* out,
+                      int64_t out_t, int64_t out_h, float* lse, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  return attention(q, q_t, q_h, k, k_t, k_h, v, v_t, v_h, cu_q, cu_k, batch, Tq, Tk, heads_q, heads_kv, D, dtype, scale,
+                   causal, out, out_t, out_h, lse, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 const char* convrot_status_string(int status) {

@@ -185,6 +185,53 @@ int convrot_gemm_grouped(const int8_t* q, int64_t ldq, const int8_t* w, int64_t 
 int convrot_silu(const void* x, void* y, int64_t n, void* stream);
 
 /*
+ * What an attention block computes between its q / k / v and out projections (no counterpart in the reference, where it
+ * is diffusers' code; call sites transformer.py:350-358).  16-bit tensors [T, H, D] are given by a base and their token
+ * and head strides in elements (multiples of 8; D contiguous; bases 16-byte aligned), so they may be slices of a wider
+ * projection.  dtype: CONVROT_BF16 or CONVROT_FP16 for every 16-bit tensor of a call.
+ *
+ * convrot_rotary_table   the table of a rotation with `axes` position axes (at most 8; time, height, width for video):
+ *                        out[t, j] = (cos, sin) of positions[t, a] * theta[a]^(-2 i / dims[a]), fp32 [rows, R / 2, 2],
+ *                        where pair j is pair i of axis a, the axes' dims[a] / 2 pairs following each other and R =
+ *                        sum dims <= 256 (dims even).  Angles in fp64.  positions [rows, axes] with leading dimension
+ *                        ld_pos, of pos_type CONVROT_POS_*; dims and theta are host arrays.
+ * convrot_qk_norm_rope   per head of q (heads_q) and k (heads_k; 0: q alone) and each of `rows` tokens:
+ *                        y = x * rsqrt(mean(x^2) + eps) * weight if norm (weights [D] or NULL, of dtype or fp32), then
+ *                        the first R channels of y turned by table row t (fp32 [rows, >= R / 2, 2], ld_table pairs
+ *                        apart, even; NULL: no rotation): pairs (2 j, 2 j + 1) if interleaved, else (j, j + R / 2);
+ *                        (a, b) -> (a cos - b sin, b cos + a sin).  fp32 throughout, one rounding.  An output may be
+ *                        its own input.  D a multiple of 8 up to 256; R a multiple of 8 (interleaved) or 16.
+ * convrot_attention      out = softmax(scale q k^T + mask) v for `batch` sequences packed behind each other: sequence b
+ *                        is rows [cu_q[b], cu_q[b + 1]) of q and out and [cu_k[b], cu_k[b + 1]) of k and v (device
+ *                        arrays of batch + 1 non-decreasing offsets; both NULL: one sequence, batch 1).  Rows of no
+ *                        sequence stay as they were.  Query head h reads key head h / (heads_q / heads_kv).  causal:
+ *                        query i of lq sees keys up to i + lk - lq.  A row that sees no key gives zeros (lse
+ *                        -infinity).  lse: fp32 [Tq, heads_q] natural log-sum-exp, or NULL.  fp32 scores, statistics
+ *                        and sums; softmax weights rounded to dtype for the product with v.  D a multiple of 8 up to
+ *                        128; heads_q / heads_kv <= 128; scale > 0.  The workspace (16-byte aligned, of
+ *                        convrot_attention_workspace_size bytes on the current device, -1 for bad sizes; 0: none)
+ *                        belongs to the call until its work is done.
+ */
+#define CONVROT_BF16 0
+#define CONVROT_FP16 1
+#define CONVROT_POS_I32 0
+#define CONVROT_POS_I64 1
+#define CONVROT_POS_F32 2
+#define CONVROT_POS_F64 3
+int convrot_rotary_table(const void* positions, int pos_type, int64_t ld_pos, int64_t rows, int axes, const int* dims,
+                         const double* theta, float* out, void* stream);
+int convrot_qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h, int heads_q,
+                         const void* k, int64_t k_t, int64_t k_h, void* k_out, int64_t ko_t, int64_t ko_h, int heads_k,
+                         int64_t rows, int D, int dtype, int norm, const void* q_weight, const void* k_weight,
+                         int weight_f32, float eps, const float* table, int64_t ld_table, int R, int interleaved,
+                         void* stream);
+int64_t convrot_attention_workspace_size(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int D);
+int convrot_attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v,
+                      int64_t v_t, int64_t v_h, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t Tq,
+                      int64_t Tk, int heads_q, int heads_kv, int D, int dtype, float scale, int causal, void* out,
+                      int64_t out_t, int64_t out_h, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * The Ulysses exchange fused into the kernels, over peer memory (no counterpart in the reference, whose all-to-all
  * is diffusers' NCCL call; call site distributed.py:88-96).  One process per GPU; every rank maps the others'
  * exchange buffers (convrot_ipc_*), so a chunk pointer below may name another GPU's memory.  At most 8 chunks.

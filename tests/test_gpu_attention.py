@@ -1,0 +1,346 @@
+"""The attention operators on the GPU against plain 64-bit formulas.
+
+Tolerances count roundings.  u = half a step of the 16-bit type, relative (bf16 2^-8, fp16 2^-11).
+
+* rotary table: fp32 cos / sin of an angle known to fp64: one rounding of the reduced angle's head (its remainder is
+  carried), sincospif's 2 units in the last place and the correction's two roundings: below 4 * 2^-23 absolute.
+* norm and rotation: fp32 steps of 2^-24 each (sum of D squares, rsqrt's 2 ulp, three products, the rotation), together
+  below (D + 16) 2^-24 of |a| + |b|, and one rounding u of the result.
+* attention: each weight p is rounded once (u) before its product with v, the result once: u (A + |o|) with
+  A = sum_k w_k |v_k|; the scores' fp32 sums are off by at most (D + 4) 2^-23 sum_d |q_d k_d| scale = e, which moves a
+  weight by a factor exp(2 e); exp2, sums, rescaling and joining in fp32 stay below 2^-17 A for the lengths used here.
+  fp16 weights below 2^-14 (of a largest of at least 1) are off by at most 2^-25 each.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from hyperflow_h3_flash_b200 import _lib
+from hyperflow_h3_flash_b200 import attention as A
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+U = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    yield
+    assert _lib.lib().convrot_poll_error(None) == 0
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(*shape, seed, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=_gen(seed), device=DEV) * scale).to(dtype)
+
+
+def _cu(lens):
+    return torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=DEV)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+
+
+def reference(q, k, v, lq, lk, causal, scale):
+    """(o, lse, bound of |o|'s error, seen rows) in fp64, by the definition, sequence by sequence and head by head."""
+    u, D = U[q.dtype], q.shape[2]
+    o = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    bound = torch.zeros_like(o)
+    lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device=DEV)
+    lse_bound = torch.zeros_like(lse)
+    group = q.shape[1] // k.shape[1]
+    q0 = k0 = 0
+    for a, b in zip(lq, lk):
+        for h in range(q.shape[1]):
+            if a and b:
+                Q = q[q0 : q0 + a, h].double()
+                K, V = (t[k0 : k0 + b, h // group].double() for t in (k, v))
+                s = Q @ K.t() * scale
+                if causal:
+                    i = torch.arange(a, device=DEV)[:, None]
+                    s = s.masked_fill(torch.arange(b, device=DEV)[None] > i + b - a, -math.inf)
+                top = s.amax(1, keepdim=True)
+                e = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
+                total = e.sum(1, keepdim=True)
+                w = e / torch.where(total == 0, 1.0, total)
+                o[q0 : q0 + a, h] = w @ V
+                lse[q0 : q0 + a, h] = (top + total.log())[:, 0]
+                size = w @ V.abs()
+                slip = (D + 4) * 2.0**-23 * (Q.abs() @ K.abs().t() * scale).amax(1, keepdim=True)
+                tiny = 2.0**-25 * V.abs().sum(0) if q.dtype == torch.float16 else 0.0
+                bound[q0 : q0 + a, h] = u * (1 + u) * (size + o[q0 : q0 + a, h].abs()) + size * (
+                    torch.expm1(2 * slip) + 2.0**-17) + tiny + 1e-30
+                lse_bound[q0 : q0 + a, h] = slip[:, 0] + 2.0**-17
+        q0, k0 = q0 + a, k0 + b
+    return o, lse, bound, lse_bound
+
+
+def check(q, k, v, lq, lk, causal=False, scale=None, cu=True, **kw):
+    scale_ = q.shape[2] ** -0.5 if scale is None else scale
+    args = {"cu_q": _cu(lq), "cu_k": _cu(lk)} if cu else {}
+    got, lse = A.attention(q, k, v, causal=causal, scale=scale, return_lse=True, **args, **kw)
+    want, want_lse, bound, lse_bound = reference(q, k, v, lq, lk, causal, scale_)
+    n = sum(lq)
+    assert got.dtype == q.dtype and got.shape == q.shape and lse.shape == q.shape[:2]
+    off = (got[:n].double() - want[:n]).abs() - bound[:n]
+    assert not torch.isnan(off).any()
+    assert (off <= 0).all(), f"{int((off > 0).sum())} of {off.numel()} outside, worst by {off.max().item():.3e}"
+    empty = want_lse[:n] == -math.inf
+    assert torch.equal(lse[:n] == -math.inf, empty)
+    assert (got[:n][empty] == 0).all()
+    d = torch.where(empty, 0.0, (lse[:n].double() - want_lse[:n]).abs())
+    assert (d <= lse_bound[:n]).all(), f"lse off by {d.max().item():.3e}"
+    return got
+
+
+def qkv(Tq, Tk, Hq, Hkv, D, dtype=torch.bfloat16, seed=0, spread=1.5):
+    return (_randn(Tq, Hq, D, seed=seed, dtype=dtype, scale=spread), _randn(Tk, Hkv, D, seed=seed + 1, dtype=dtype),
+            _randn(Tk, Hkv, D, seed=seed + 2, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [8, 16, 40, 64, 72, 80, 96, 120, 128])
+def test_head_dims_and_types(D, dtype):
+    q, k, v = qkv(300, 333, 2, 2, D, dtype, seed=D)
+    check(q, k, v, [300], [333], cu=False)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lq,lk", [(1, 1), (1, 128), (1, 129), (127, 127), (128, 128), (129, 255), (255, 129), (256, 256),
+                                   (257, 640), (17, 1025), (500, 7), (640, 1)])
+def test_lengths(lq, lk, causal):
+    q, k, v = qkv(lq, lk, 3, 3, 64, seed=lq + lk)
+    check(q, k, v, [lq], [lk], causal, cu=False)
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 8, 40, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_grouped_heads(group, causal):
+    q, k, v = qkv(70, 200, 2 * group, 2, 64, seed=group)
+    check(q, k, v, [70], [200], causal, cu=False)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_packed_sequences(causal, dtype):
+    lq = [130, 0, 1, 257, 64, 5, 0]
+    lk = [131, 9, 0, 300, 63, 700, 0]
+    q, k, v = qkv(sum(lq), sum(lk), 4, 2, 128, dtype, seed=3)
+    check(q, k, v, lq, lk, causal)
+
+
+def test_many_sequences():
+    """More sequences than one warp looks at in a step, empty ones among them."""
+    lq = [(7 * i) % 5 for i in range(101)]
+    lk = [(13 * i) % 150 for i in range(101)]
+    q, k, v = qkv(sum(lq), sum(lk), 4, 2, 64, seed=4)
+    check(q, k, v, lq, lk, True)
+
+
+@pytest.mark.parametrize("lk", [[2000], [1, 5000, 300, 0, 129]])
+@pytest.mark.parametrize("new", [1, 3])
+def test_single_tokens_over_long_keys(lk, new):
+    lq = [new] * len(lk)
+    q, k, v = qkv(sum(lq), sum(lk), 10, 2, 128, seed=5)
+    assert _lib.lib().convrot_attention_workspace_size(sum(lq), sum(lk), len(lk), 10, 2, 128) > 0  # keys are split
+    check(q, k, v, lq, lk, True)
+
+
+def test_scores_that_grow_and_shrink_along_the_keys():
+    """Maxima that jump by far more than the lazy rescaling's step, up and down, and rows of equal scores."""
+    q, k, v = qkv(200, 1500, 2, 2, 64, seed=6, spread=1.0)
+    ramp = torch.linspace(-6, 6, 1500, device=DEV).reshape(-1, 1, 1)
+    k = (k + ramp * q.float().mean(0) * 20).to(k.dtype)
+    check(q, k, v, [200], [1500], cu=False)
+    check(q, k.flip(0).contiguous(), v, [200], [1500], cu=False)
+    check(torch.zeros_like(q), k, v, [200], [1500], cu=False)
+    check(q, k, v, [200], [1500], cu=False, scale=3.0)
+
+
+def test_strided_views_of_a_fused_projection():
+    T, Hq, Hkv, D = 311, 6, 2, 64
+    x = _randn(T, (Hq + 2 * Hkv) * D + 8, seed=7, dtype=torch.bfloat16)
+    q = x[:, : Hq * D].unflatten(1, (Hq, D))
+    k = x[:, Hq * D : (Hq + Hkv) * D].unflatten(1, (Hkv, D))
+    v = x[:, (Hq + Hkv) * D : (Hq + 2 * Hkv) * D].unflatten(1, (Hkv, D))
+    check(q, k, v, [T], [T], True, cu=False)
+    heads_first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    out = torch.empty(Hq, T, D, dtype=q.dtype, device=DEV).transpose(0, 1)
+    check(*heads_first, [T], [T], True, cu=False, out=out)
+
+
+def test_rows_of_no_sequence_stay_as_they_were():
+    lq, lk = [100, 50], [60, 90]
+    q, k, v = qkv(200, 300, 2, 2, 64, seed=8)
+    out = torch.full_like(q, 7.0)
+    A.attention(q, k, v, cu_q=_cu(lq), cu_k=_cu(lk), out=out)
+    assert (out[150:] == 7).all() and not (out[:150] == 7).all()
+    few = torch.full_like(q[:9], 7.0)
+    A.attention(q[:9], k, v, cu_q=_cu([1, 1, 2]), cu_k=_cu([60, 90, 100]), out=few)
+    assert (few[4:] == 7).all() and not (few[:4] == 7).any()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_what_no_query_sees_does_not_reach_it(bad):
+    """Rows behind a sequence (another request's, or padding) hold NaN or infinities."""
+    lq, lk = [130, 40], [130, 70]
+    q, k, v = qkv(sum(lq) + 60, sum(lk) + 60, 2, 2, 128, seed=9)
+    clean = check(q, k, v, lq, lk)
+    for t, n in ((q, sum(lq)), (k, sum(lk)), (v, sum(lk))):
+        t[n:] = bad
+    got = A.attention(q, k, v, cu_q=_cu(lq), cu_k=_cu(lk))
+    assert torch.equal(got[: sum(lq)], clean[: sum(lq)])
+    # another request's rows: sequence 1 is spoilt, sequence 0 is not
+    for t, n in ((q, lq[0]), (k, lk[0]), (v, lk[0])):
+        t[n:] = bad
+    got = A.attention(q, k, v, cu_q=_cu(lq), cu_k=_cu(lk))
+    assert torch.equal(got[: lq[0]], clean[: lq[0]])
+
+
+def test_offsets_that_make_no_sense_stay_inside():
+    q, k, v = qkv(64, 64, 2, 2, 64, seed=10)
+    for cu in ([0, 1000, 64], [-5, 30, 64], [50, 20, 64]):
+        cu = torch.tensor(cu, dtype=torch.int32, device=DEV)
+        A.attention(q, k, v, cu_q=cu, cu_k=cu)
+    torch.cuda.synchronize()
+
+
+def test_results_repeat_bitwise():
+    lk = [3000, 17, 900]
+    q, k, v = qkv(3, sum(lk), 8, 2, 128, seed=11)
+    args = {"cu_q": _cu([1, 1, 1]), "cu_k": _cu(lk)}
+    first = A.attention(q, k, v, **args)
+    for _ in range(5):
+        assert torch.equal(A.attention(q, k, v, **args), first)
+
+
+def test_empty_calls():
+    q, k, v = qkv(0, 10, 2, 2, 64)
+    assert A.attention(q, k, v).shape == (0, 2, 64)
+    q, k, v = qkv(5, 0, 2, 2, 64)
+    o, lse = A.attention(q, k, v, return_lse=True)
+    assert (o == 0).all() and (lse == -math.inf).all()
+    o = A.attention(q, k, v, cu_q=torch.zeros(1, dtype=torch.int32, device=DEV),
+                    cu_k=torch.zeros(1, dtype=torch.int32, device=DEV), out=torch.ones_like(q))
+    assert (o == 1).all()
+
+
+# ------------------------------------------------------------------------------------------------ rotary table
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64, torch.float32, torch.float64])
+@pytest.mark.parametrize("axes,theta", [((2,), 10000.0), ((128,), 10000.0), ((44, 42, 42), 10000.0), ((16, 24, 24), (100.0, 1e4, 5e5)),
+                                        ((64, 32, 32, 64, 64), 256.0)])
+def test_rotary_table(axes, theta, dtype):
+    T = 777
+    pos = torch.randint(0, 2_000_000, (T, len(axes)), generator=_gen(1), device=DEV).double()
+    pos[:40] = torch.arange(40, device=DEV, dtype=torch.float64)[:, None]
+    if dtype.is_floating_point:
+        pos = pos * 0.37 - 1000
+    pos = pos.to(dtype)
+    table = A.rotary_table(pos, axes, theta=theta)
+    thetas = theta if isinstance(theta, tuple) else (theta,) * len(axes)
+    ang = torch.cat([pos[:, a, None].double() * (thetas[a] ** (-torch.arange(0, d, 2, device=DEV).double() / d))
+                     for a, d in enumerate(axes)], dim=1)
+    want = torch.stack([ang.cos(), ang.sin()], dim=-1)
+    assert table.shape == (T, sum(axes) // 2, 2) and table.dtype == torch.float32
+    # fp64 angles of 2e6 are themselves known to 2e6 * 2^-52
+    assert (table.double() - want).abs().max() <= 4 * 2.0**-23 + 2e6 * 2.0**-51
+
+
+def test_rotary_table_of_strided_and_few_positions():
+    pos = torch.randint(0, 50, (30, 5), generator=_gen(2), device=DEV, dtype=torch.int32)
+    assert torch.equal(A.rotary_table(pos[:, 1:4], (16, 24, 24)), A.rotary_table(pos[:, 1:4].contiguous(), (16, 24, 24)))
+    assert torch.equal(A.rotary_table(pos[:, 2], (64,)), A.rotary_table(pos[:, 2:3].contiguous(), (64,)))
+    assert torch.equal(A.rotary_table(pos[:1, 1:4].expand(30, 3), (16, 24, 24))[29],
+                       A.rotary_table(pos[:1, 1:4].contiguous(), (16, 24, 24))[0])
+    assert A.rotary_table(pos[:0, :3], (16, 24, 24)).shape == (0, 32, 2)
+    assert torch.isnan(A.rotary_table(torch.tensor([math.inf, math.nan], device=DEV), (8,))).all()
+
+
+# ------------------------------------------------------------------------------------------------ norm and rotation
+
+
+def norm_rope_reference(x, weight, eps, norm, table, interleaved):
+    """(y, bound) in fp64."""
+    y = x.double()
+    D = x.shape[2]
+    if norm:
+        y = y / torch.sqrt(y.square().mean(-1, keepdim=True) + eps)
+        if weight is not None:
+            y = y * weight.double()
+    size = y.abs()
+    if table is not None:
+        R = 2 * table.shape[1]
+        c, s = table.double()[:, None, :, 0], table.double()[:, None, :, 1]
+        sel = (slice(0, R, 2), slice(1, R, 2)) if interleaved else (slice(0, R // 2), slice(R // 2, R))
+        a, b = y[..., sel[0]].clone(), y[..., sel[1]].clone()
+        y[..., sel[0]], y[..., sel[1]] = a * c - b * s, b * c + a * s
+        size[..., sel[0]] = size[..., sel[1]] = a.abs() + b.abs()
+    step = (D + 16) * 2.0**-24 * size
+    return y, U[x.dtype] * (y.abs() + step) + step + 2.0**-25 * (x.dtype == torch.float16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("D,R", [(8, 8), (16, 16), (40, 32), (64, 64), (72, 48), (80, 80), (128, 128), (128, 64), (200, 160),
+                                 (256, 256)])
+def test_norm_and_rotation(D, R, interleaved, dtype):
+    if R % 16 and not interleaved:
+        R = None
+    T, Hq, Hk = 37, 5, 3
+    q = _randn(T, Hq, D, seed=D, dtype=dtype, scale=3.0)
+    k = _randn(T, Hk, D, seed=D + 1, dtype=dtype, scale=0.1)
+    q[0, 0] = 0
+    table = None if R is None else A.rotary_table(torch.arange(T, device=DEV) * 97, (R,))
+    for norm, weights in ((True, dtype), (True, torch.float32), (True, None), (False, None)):
+        if not norm and table is None:
+            continue
+        wq, wk = (None, None) if weights is None else (1 + _randn(D, seed=1, scale=0.3), 1 + _randn(D, seed=2, scale=0.3))
+        if weights is not None:
+            wq, wk = wq.to(weights), wk.to(weights)
+        got = A.qk_norm_rope(q, k, q_weight=wq, k_weight=wk, eps=1e-5, norm=norm, table=table, interleaved=interleaved)
+        for g, x, w in zip(got, (q, k), (wq, wk)):
+            want, bound = norm_rope_reference(x, w, 1e-5, norm, table, interleaved)
+            assert g.dtype == dtype and ((g.double() - want).abs() <= bound).all()
+        alone = A.qk_norm_rope(q, q_weight=wq, eps=1e-5, norm=norm, table=table, interleaved=interleaved)
+        assert torch.equal(alone, got[0])
+
+
+@pytest.mark.parametrize("T", [0, 1, 2, 1000])
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (7, 1), (40, 40), (3, 40)])
+def test_norm_and_rotation_of_any_rows_in_place_and_strided(T, Hq, Hk):
+    D = 64
+    x = _randn(T, (Hq + 2 * Hk) * D, seed=5, dtype=torch.bfloat16)
+    q, k = x[:, : Hq * D].unflatten(1, (Hq, D)), x[:, Hq * D : (Hq + Hk) * D].unflatten(1, (Hk, D))
+    w = 1 + _randn(D, seed=6, dtype=torch.bfloat16, scale=0.3)
+    table = A.rotary_table(torch.arange(T, device=DEV), (48,))
+    rest = x[:, (Hq + Hk) * D :].clone()
+    args = {"q_weight": w, "k_weight": w, "table": table}
+    fresh = A.qk_norm_rope(q.contiguous(), k.contiguous(), **args)
+    outs = A.qk_norm_rope(q, k, **args)
+    assert torch.equal(outs[0], fresh[0]) and torch.equal(outs[1], fresh[1])
+    for g, t in zip(fresh, (q, k)):
+        want, bound = norm_rope_reference(t, w, 1e-6, True, table, True)
+        assert ((g.double() - want).abs() <= bound).all()
+    back = A.qk_norm_rope(q, k, q_out=q, k_out=k, **args)
+    assert back[0] is q and torch.equal(q, fresh[0]) and torch.equal(k, fresh[1])
+    assert torch.equal(x[:, (Hq + Hk) * D :], rest)
+
+
+def test_rows_of_nan_stay_in_their_head():
+    q = _randn(4, 4, 128, seed=7, dtype=torch.bfloat16)
+    clean = A.qk_norm_rope(q)
+    q[1, 2, 5] = math.nan
+    got = A.qk_norm_rope(q)
+    assert torch.isnan(got[1, 2]).all()
+    got[1, 2] = clean[1, 2]
+    assert torch.equal(got, clean)
