@@ -344,3 +344,27 @@ def test_rows_of_nan_stay_in_their_head():
     assert torch.isnan(got[1, 2]).all()
     got[1, 2] = clean[1, 2]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("lk", [70, 300])
+def test_scores_that_are_not_finite(lk):
+    """NaN and +infinity among a row's scores make the row NaN, -infinity a weight of zero; other rows do not change."""
+    q, k, v = qkv(140, lk, 2, 2, 64, seed=12)
+    q = q.abs() + 0.1
+    clean = A.attention(q, k, v)
+    for key in range(0, lk, 11):
+        bad = k.clone()
+        bad[key, 0, 3] = -math.inf
+        want, *_ = reference(q, bad, v, [140], [lk], False, 0.125)
+        got = A.attention(q, bad, v)
+        assert not torch.isnan(got).any() and torch.equal(got[:, 1], clean[:, 1])
+        assert (got.double() - want).abs().max() <= 0.03
+        bad[key, 0, 3] = math.inf if key % 2 else math.nan
+        got = A.attention(q, bad, v)
+        assert torch.isnan(got[:, 0]).all() and torch.equal(got[:, 1], clean[:, 1])
+    row = q.clone()
+    row[77, 1] = math.nan
+    got = A.attention(row, k, v)
+    assert torch.isnan(got[77, 1]).all()
+    got[77, 1] = clean[77, 1]
+    assert torch.equal(got, clean)
