@@ -39,15 +39,18 @@ constexpr int kAtThreads = 384;
 constexpr int kAtPanelBytes = 128 * 128;  // 128 rows x 64 channels of 16 bits, 128-byte swizzled rows
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kFirstSteps = 6;  // 16-key steps of a tile's weights that are handed over before the rest
-constexpr int kPolyEvery = 1000;  // one of so many pairs of weights takes exp2_poly instead of the special-function unit
+
+constexpr int kItems = 4;        // items on their way through the CTA
+constexpr int kMaxShares = 192;  // most CTAs that share the last items evenly
 
 template <int NP>
 struct AttnCfg {  // NP: 64-channel panels of a head (1: D <= 64, 2: D <= 128)
   static constexpr int kTileBytes = NP * kAtPanelBytes;
   static constexpr int kStages = NP == 2 ? 5 : 8;
-  static constexpr int kNumBars = 2 * kStages + 2 + 2 + 2 + 4 + 2 + 3;
-  static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 8 * kNumBars + 16 + 1024;
-  static constexpr int kO = 256;  // first TMEM column of O0; O1 follows NP * 64 columns later
+  static constexpr int kNumBars = 2 * kStages + 20 + 2 * kItems;
+  static constexpr int kSmallBytes = 8 * kNumBars + kItems * 48 + 2 * 16 + 4 * (kMaxShares + 1) + 16;
+  static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + kSmallBytes + 1024;
+  static constexpr int kO = 256;  // TMEM columns from S_i to O_i
 };
 
 struct AttnParams {
@@ -61,22 +64,42 @@ struct AttnParams {
   void* out;
   int64_t out_t, out_h;
   float* lse;  // [Tq, heads] or null
-  // Split keys: sequence b's tiles are divided into ceil(tiles / chunk_tiles) parts, at most max_splits; each part
-  // writes its normalised rows and their log2-sum-exp, joined by attention_combine_kernel.
-  int max_splits, chunk_tiles;
-  float* part_o;    // [max_splits, Tq, heads, D]
-  float* part_lse;  // [max_splits, Tq, heads]
+  // shares > 0: the items that do not fill a whole wave of `shares` CTAs are divided evenly by key tiles, and what is
+  // not a whole item goes to part_o / part_lse, joined by attention_combine_kernel.
+  int shares;
+  int* meta;        // [kMaxShares + 4]: shares in use, items, first item, prefix of the items' work
+  float* part_o;    // [2 shares, 256, D] normalised rows
+  float* part_lse;  // [2 shares, 256] log2-sum-exp
   uint64_t wait_limit_ns;
   int* error_word;
 };
 
 // ------------------------------------------------------------------------------------------------ work items
+//
+// An item is two neighbouring query tiles of one key head of one sequence, with all of its key tiles.  The grid has one
+// CTA for each; a resident CTA's scheduler warp (11) finds its item in the offset arrays, hands it to the other warps
+// through shared memory, and then takes over the next CTA that has not been launched (cluster launch control): dynamic
+// balance without a counter in memory, no start-up between items, and the loads of the next item begin while the last
+// tiles of this one are multiplied.  Causal items come longest first within a head.
+//
+// Where the last wave of items would leave SMs idle, its items are divided evenly (AttnParams::shares): share s of G gets
+// the s-th G-th of their key tiles, whichever items these lie in.  32760 tokens x 5 heads are 640 items on 148 SMs, 5
+// waves for 4.3 waves of work.
+//
+// An item of a single query tile (a sequence's last one, or a few new tokens over a long cache) uses both softmax
+// groups all the same: tile 0 takes the even key tiles and tile 1 the odd ones, each with its own m, l and o, joined at
+// the end ("twin").
 
 struct AttnItem {
-  int q0, lq, k0, lk;  // the sequence's rows
-  int head;            // key head
-  int pos;             // first query position of the item (two tiles of `positions`)
-  int split, t_lo, t_hi;  // key tiles [t_lo, t_hi) of this split
+  int q_row, left;  // first row of q and out; query positions from there to the sequence's end
+  int k_row, keys;  // first row of k and v; keys from there to the sequence's end
+  int head;         // key head
+  int see;          // keys from k_row that the first position sees (position r: r more, if causal)
+  int nt[2];        // key tiles of each query tile
+  int twin;         // tile 1 is tile 0 again
+  int fixing;       // the last value tile has rows of another sequence
+  int part;         // slot of the partial result, or -1
+  int valid;        // 0: no more work
 };
 
 __device__ __forceinline__ void attn_bounds(const int32_t* cu, int b, int total, int& begin, int& len) {
@@ -91,29 +114,54 @@ __device__ __forceinline__ void attn_bounds(const int32_t* cu, int b, int total,
   len = min(max(__ldg(cu + b + 1), lo), total) - lo;
 }
 
-__device__ __forceinline__ int attn_splits(const AttnParams& p, int lk) {
-  if (p.max_splits <= 1) return 1;
-  const int tiles = (lk + kAtTile - 1) / kAtTile;
-  return min(p.max_splits, max(1, (tiles + p.chunk_tiles - 1) / p.chunk_tiles));
+// A sequence and an item's place in it.
+struct AttnPlace {
+  int q0, lq, k0, lk, head, pos;
+};
+
+// Key tiles that the query tile beginning at position `first` needs.
+__device__ __forceinline__ int attn_tiles(const AttnParams& p, const AttnPlace& a, int first) {
+  if (first >= a.lq) return 0;
+  const int last = min(first + p.positions, a.lq) - 1;
+  const int limit = p.causal ? min(a.lk, last + a.lk - a.lq + 1) : a.lk;
+  return limit <= 0 ? 0 : (limit + kAtTile - 1) / kAtTile;
 }
 
-// Finds items in increasing order; the whole warp calls next().  (base, b) is the first item and the index of the block
-// of 32 sequences last looked at.
+// An item's place from its number within its sequence.
+__device__ __forceinline__ void attn_place(const AttnParams& p, int local, AttnPlace& a) {
+  const int span = 2 * p.positions;
+  const int nq = (a.lq + span - 1) / span;
+  a.head = local / nq;
+  const int qt = local - a.head * nq;
+  a.pos = (p.causal ? nq - 1 - qt : qt) * span;
+}
+
+// Work of an item in units of one 128 x 128 tile: a step of a pair of tiles counts two.
+__device__ __forceinline__ int attn_unit(const AttnParams& p, const AttnPlace& a) {
+  return a.lq - a.pos > p.positions ? 2 : 1;
+}
+__device__ __forceinline__ int attn_work(const AttnParams& p, const AttnPlace& a) {
+  const int n = max(attn_tiles(p, a, a.pos), attn_tiles(p, a, a.pos + p.positions));
+  return max(n, 1) * attn_unit(p, a);
+}
+
+// Finds items by number; the whole warp calls find().  (base, block) is the number of the first item of the 32 sequences
+// last looked at.
 struct AttnWalk {
   int base = 0;
   int block = 0;
 
-  __device__ __forceinline__ bool find(const AttnParams& p, int item, int lane, AttnItem& it) {
+  __device__ __forceinline__ bool find(const AttnParams& p, int item, int lane, AttnPlace& a) {
+    if (item < base) base = block = 0;
     const int span = 2 * p.positions;
     while (block < p.batch) {
       const int b = block + lane;
       int q0 = 0, lq = 0, k0 = 0, lk = 0;
-      int mine = 0;
       if (b < p.batch) {
         attn_bounds(p.cu_q, b, p.Tq, q0, lq);
         attn_bounds(p.cu_k, b, p.Tk, k0, lk);
-        mine = (lq + span - 1) / span * attn_splits(p, lk) * p.heads_kv;
       }
+      const int mine = (lq + span - 1) / span * p.heads_kv;
       int upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -128,39 +176,49 @@ struct AttnWalk {
         continue;
       }
       const int src = __ffs(after) - 1;
-      it.q0 = __shfl_sync(0xffffffffu, q0, src);
-      it.lq = __shfl_sync(0xffffffffu, lq, src);
-      it.k0 = __shfl_sync(0xffffffffu, k0, src);
-      it.lk = __shfl_sync(0xffffffffu, lk, src);
-      const int local = rel - __shfl_sync(0xffffffffu, upto - mine, src);
-      const int ns = attn_splits(p, it.lk);
-      const int nq = (it.lq + span - 1) / span;
-      const int per_head = ns * nq;
-      it.head = local / per_head;
-      const int in_head = local - it.head * per_head;
-      int qt = in_head / ns;
-      it.split = in_head - qt * ns;
-      if (p.causal) qt = nq - 1 - qt;  // the longest first
-      it.pos = qt * span;
-      const int tiles = (it.lk + kAtTile - 1) / kAtTile;
-      const int per = (tiles + ns - 1) / ns;
-      it.t_lo = min(it.split * per, tiles);
-      it.t_hi = min(it.t_lo + per, tiles);
+      a.q0 = __shfl_sync(0xffffffffu, q0, src);
+      a.lq = __shfl_sync(0xffffffffu, lq, src);
+      a.k0 = __shfl_sync(0xffffffffu, k0, src);
+      a.lk = __shfl_sync(0xffffffffu, lk, src);
+      attn_place(p, rel - __shfl_sync(0xffffffffu, upto - mine, src), a);
       return true;
     }
     return false;
   }
 };
 
-// Keys that the last position of query tile i sees, and the key tiles of this split that it needs.
-__device__ __forceinline__ int attn_tiles(const AttnParams& p, const AttnItem& it, int i) {
-  const int first = it.pos + i * p.positions;
-  if (first >= it.lq) return 0;
-  const int last = min(first + p.positions, it.lq) - 1;
-  const int limit = p.causal ? min(it.lk, last + it.lk - it.lq + 1) : it.lk;
-  const int tiles = limit <= 0 ? 0 : (limit + kAtTile - 1) / kAtTile;
-  return max(0, min(tiles, it.t_hi) - it.t_lo);
+// All items of the call.
+__device__ __forceinline__ int attn_count(const AttnParams& p, int lane) {
+  const int span = 2 * p.positions;
+  int n = 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    int q0, lq;
+    attn_bounds(p.cu_q, b, p.Tq, q0, lq);
+    n += (lq + span - 1) / span;
+  }
+  return __reduce_add_sync(0xffffffffu, n) * p.heads_kv;
 }
+
+// Even division of the last items.  pre[x] is the work before item x of them (`items` of them, `total` in all); share s
+// of `shares` begins at edge(s): at a whole step of the item that it falls into, or at that item's edge if little would
+// be cut off.
+struct AttnShares {
+  const int* pre;
+  int items, total, shares;
+
+  __device__ __forceinline__ int item_at(int x, int lane) const {  // the item that work unit x < total lies in
+    int n = 0;
+    for (int i = 0; i < items; i += 32)
+      n += __popc(__ballot_sync(0xffffffffu, i + lane < items && pre[i + lane + 1] <= x));
+    return n;
+  }
+  __device__ __forceinline__ int edge(int s, int unit_of_item, int i) const {
+    const int x = static_cast<int>(static_cast<int64_t>(total) * s / shares);
+    const int a = pre[i], e = pre[i + 1];
+    if (x - a < 4 || e - x < 4) return x - a < e - x ? a : e;
+    return a + (x - a + unit_of_item - 1) / unit_of_item * unit_of_item;
+  }
+};
 
 // ------------------------------------------------------------------------------------------------ small wrappers
 
@@ -237,9 +295,14 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {  // wi
 }
 
 struct AttnGuard {
-  volatile int* abort;
-  uint64_t limit_ns;
-  int* error_word;
+  uint32_t abort;  // shared address of the flag
+  const AttnParams& p;
+
+  __device__ __forceinline__ bool aborted() const {
+    int v;
+    asm volatile("ld.volatile.shared.s32 %0, [%1];" : "=r"(v) : "r"(abort) : "memory");
+    return v != 0;
+  }
 
   __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) const {
     if (bar_try(bar, parity)) return;
@@ -263,12 +326,12 @@ struct AttnGuard {
     uint64_t since = 0;
     for (uint32_t spin = 1; !bar_try(bar, parity); ++spin) {
       if (spin & 127) continue;
-      if (*abort) return;
+      if (aborted()) return;
       const uint64_t now = globaltimer_ns();
       if (since == 0) since = now;
-      if (now - since > limit_ns) {
-        *abort = 1;
-        if (error_word) atomicCAS(error_word, 0, 6 /* CONVROT_ERR_TIMEOUT */);
+      if (now - since > p.wait_limit_ns) {
+        asm volatile("st.volatile.shared.s32 [%0], 1;" ::"r"(abort) : "memory");
+        if (p.error_word) atomicCAS(p.error_word, 0, 6 /* CONVROT_ERR_TIMEOUT */);
         return;
       }
     }
@@ -315,6 +378,38 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st_32x32b_x2(uint32_t taddr, uint32_t a, uint32_t b) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(a), "r"(b) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_32x32b_x2(uint32_t taddr, uint32_t& a, uint32_t& b) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(taddr) : "memory");
+}
+
+// Asks for the next CTA of the grid that has not been launched; the 16-byte answer arrives on `bar`.
+__device__ __forceinline__ void launch_cancel(uint32_t answer, uint32_t bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer),
+      "r"(bar)
+      : "memory");
+}
+
+// blockIdx.x of the CTA that was taken over, or -1 if none is left.
+__device__ __forceinline__ int launch_cancelled(uint32_t answer) {
+  int got, x = -1;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.s32 %0, 1, 0, p;\n\t"
+      "mov.s32 %1, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(answer)
+      : "memory");
+  return got ? x : -1;
+}
+
 // Two fp32 lanes in a 64-bit register (one issue slot for both).
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t d;
@@ -337,27 +432,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// 2^x of two lanes on the FMA pipe: x = n + f with n = rint(x) (by adding and subtracting 1.5 * 2^23, which leaves n in
-// the low bits of the sum) and |f| <= 1/2, 2^f = 1 + f q(f) with a cubic q fitted to the smallest largest relative error
-// (2.9e-6, far below the 16-bit rounding of the weights), and n added to the exponent.  x is below 2^7 and not NaN (a
-// row with a NaN score has a NaN maximum, and the special-function lanes carry it); at -127 and below, -infinity
-// included, the result is exactly 0.
-__device__ __forceinline__ float2 exp2_poly(uint64_t x) {
-  const float2 v = unpack2(x);
-  const uint64_t xc = pack2(fmaxf(v.x, -127.0f), fmaxf(v.y, -127.0f));
-  const uint64_t t = add2(xc, pack2(12582912.0f, 12582912.0f));
-  const uint64_t n = add2(t, pack2(-12582912.0f, -12582912.0f));
-  const uint64_t f = fma2(n, pack2(-1.0f, -1.0f), xc);
-  uint64_t q = fma2(f, pack2(0.0095828531f, 0.0095828531f), pack2(0.055906427f, 0.055906427f));
-  q = fma2(q, f, pack2(0.24024099f, 0.24024099f));
-  q = fma2(q, f, pack2(0.69312419f, 0.69312419f));
-  q = fma2(q, f, pack2(1.0f, 1.0f));
-  const float2 y = unpack2(q), k = unpack2(t);
-  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(k.x) << 23)),
-                     __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(k.y) << 23)));
-}
-
-// Weights 2^(c2 s + neg) of 32 scores, their sums (two lanes of two), and the weights in 16 bits.
+// Weights 2^(c2 s + neg) of 32 scores, their sums (two lanes of two), and the weights in 16 bits.  All of them on the
+// special-function unit: one in 2, 3, 4, 8 or 16 of them by a quartic on the FMA pipe shortened this step, but the
+// kernel took 3 to 13 % longer at 128 channels (more issue slots beside the MMA warp, and a lower clock under the power
+// limit) and gained nothing at 64.
 template <class T>
 __device__ __forceinline__ void weights(const uint32_t (&s)[32], float c2, float neg, uint64_t (&sum)[2],
                                         uint32_t (&pk)[16]) {
@@ -365,13 +443,8 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], float c2, float
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const uint64_t x = fma2(pack2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale2, neg2);
-    float2 y;
-    if (e % kPolyEvery == kPolyEvery - 1) {
-      y = exp2_poly(x);
-    } else {
-      const float2 v = unpack2(x);
-      y = make_float2(exp2_approx(v.x), exp2_approx(v.y));
-    }
+    const float2 v = unpack2(x);
+    const float2 y = make_float2(exp2_approx(v.x), exp2_approx(v.y));
     sum[e & 1] = add2(sum[e & 1], pack2(y.x, y.y));
     pk[e] = Pack16<T>::pack(y.x, y.y);
   }
@@ -390,8 +463,12 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(attn_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_smem = smem;                      // two query tiles
   uint8_t* ring = smem + 2 * Cfg::kTileBytes;  // key and value tiles in turn
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + S * Cfg::kTileBytes);
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
+  uint8_t* small = ring + S * Cfg::kTileBytes;
+  AttnItem* item_smem = reinterpret_cast<AttnItem*>(small);              // [kItems]
+  const uint32_t answers = smem_u32(small + kItems * sizeof(AttnItem));       // [2] of launch control
+  uint64_t* bars = reinterpret_cast<uint64_t*>(small + kItems * sizeof(AttnItem) + 32);
+  int* pre = reinterpret_cast<int*>(bars + Cfg::kNumBars);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pre + kMaxShares + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   const uint32_t bar0 = smem_u32(bars);
   auto kv_full = [&](int s) { return bar0 + 8 * s; };
@@ -401,15 +478,25 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   auto s_full = [&](int i) { return bar0 + 8 * (2 * S + 4 + i); };  // scores of tile i (and all products before) done
   auto o_full = [&](int i) { return bar0 + 8 * (2 * S + 6 + i); };  // tile i's last product of the item done
   auto p_full = [&](int i, int part) { return bar0 + 8 * (2 * S + 8 + 2 * i + part); };  // weights of tile i in TMEM
-  const uint32_t v_need = bar0 + 8 * (2 * S + 12);   // a value tile with rows behind the sequence has arrived
-  const uint32_t v_fixed = bar0 + 8 * (2 * S + 13);  // and those rows are cleared
+  const uint32_t v_need = bar0 + 8 * (2 * S + 12);      // a value tile with rows behind the sequence has arrived
+  const uint32_t v_fixed = bar0 + 8 * (2 * S + 13);     // and those rows are cleared
   const uint32_t drain = bar0 + 8 * (2 * S + 14);
+  const uint32_t twin_ready = bar0 + 8 * (2 * S + 15);  // tile 1's part of a twin item is in TMEM
+  const uint32_t twin_done = bar0 + 8 * (2 * S + 16);   // and was read
+  const uint32_t want = bar0 + 8 * (2 * S + 17);        // the producer has issued all loads of its item
+  auto answer_full = [&](int i) { return bar0 + 8 * (2 * S + 18 + i); };
+  auto item_full = [&](int i) { return bar0 + 8 * (2 * S + 20 + i); };
+  auto item_empty = [&](int i) { return bar0 + 8 * (2 * S + 20 + kItems + i); };
+  constexpr int kReaders = 11;                          // warps that read an item: all but the scheduler
 
   const int warp = uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int b = 0; b < Cfg::kNumBars; ++b) mbar_init(&bars[b], b >= 2 * S + 8 && b < 2 * S + 12 ? 4 : 1);
+    for (int b = 0; b < Cfg::kNumBars; ++b) {
+      const int c = b - 2 * S;
+      mbar_init(&bars[b], (c >= 8 && c < 12) || c == 15 || c == 16 ? 4 : c >= 20 + kItems ? kReaders : 1);
+    }
     *abort_flag = 0;
     fence_mbarrier_init();
     tma_prefetch_desc(&tmap_q);
@@ -424,39 +511,202 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(*tmem_holder);
-  const AttnGuard guard{abort_flag, p.wait_limit_ns, p.error_word};
-  AttnWalk walk;
+  const AttnGuard guard{smem_u32(const_cast<int*>(abort_flag)), p};
+
+  // The next item, in every reading warp; false at the end of the work (or after a failed wait).  The warp is done with
+  // the item's place in shared memory once it calls release().
+  uint32_t item_count = 0;
+  AttnItem* item = nullptr;
+  auto next_item = [&]() {
+    const int at = item_count % kItems;
+    guard.wait(item_full(at), (item_count / kItems) & 1);
+    item = item_smem + at;
+    return uniform(item->valid) != 0 && !guard.aborted();
+  };
+  auto release = [&]() {
+    __syncwarp();
+    if (lane == 0) bar_arrive(item_empty(item_count % kItems));
+    ++item_count;
+  };
   AttnItem it;
+  auto copy_item = [&]() {  // for the warps that need most of it
+    const int4* src = reinterpret_cast<const int4*>(item);
+    const int4 x = src[0], y = src[1], z = src[2];
+    it.q_row = uniform(x.x), it.left = uniform(x.y), it.k_row = uniform(x.z), it.keys = uniform(x.w);
+    it.head = uniform(y.x), it.see = uniform(y.y), it.nt[0] = uniform(y.z), it.nt[1] = uniform(y.w);
+    it.twin = uniform(z.x), it.fixing = uniform(z.y), it.part = uniform(z.z), it.valid = uniform(z.w);
+    release();
+  };
 
   if (warp >= 8) {
-    setmaxnreg_dec<72>();
-    if (warp == 9) {
+    setmaxnreg_dec<56>();
+    if (warp == 11) {
+      // -------------------------------------------------------------- scheduler
+      AttnWalk walk;
+      AttnPlace a;
+      const int items = attn_count(p, lane);
+      const int whole = p.shares > 0 ? items / p.shares * p.shares : items;
+      AttnShares sh{pre, items - whole, 0, 0};
+      uint32_t sent = 0, asked = 0;
+      auto send = [&](const AttnItem& x) {
+        const int at = sent % kItems;
+        guard.wait(item_empty(at), ((sent / kItems) & 1) ^ 1);
+        if (sent > 0) guard.wait(want, (sent - 1) & 1);
+        if (lane == 0) {
+          int4* dst = reinterpret_cast<int4*>(item_smem + at);
+          dst[0] = make_int4(x.q_row, x.left, x.k_row, x.keys);
+          dst[1] = make_int4(x.head, x.see, x.nt[0], x.nt[1]);
+          dst[2] = make_int4(x.twin, x.fixing, x.part, x.valid);
+          bar_arrive(item_full(at));  // releases the stores above
+        }
+        __syncwarp();
+        ++sent;
+      };
+      // steps [lo, hi) of the item at place a, as part `part` or as a whole (-1)
+      auto send_steps = [&](int lo, int hi, int part) {
+        AttnItem x;
+        const int n0 = attn_tiles(p, a, a.pos), n1 = attn_tiles(p, a, a.pos + p.positions);
+        const int first = lo * kAtTile;
+        x.q_row = a.q0 + a.pos;
+        x.left = a.lq - a.pos;
+        x.k_row = a.k0 + first;
+        x.keys = a.lk - first;
+        x.head = a.head;
+        x.see = (p.causal ? a.pos + a.lk - a.lq + 1 : a.lk) - first;
+        x.nt[0] = max(min(n0, hi) - lo, 0);
+        x.nt[1] = max(min(n1, hi) - lo, 0);
+        x.twin = x.left <= p.positions && x.nt[0] > 1;
+        const int n = max(x.nt[0], x.nt[1]);
+        x.fixing = n > 0 && n * kAtTile > x.keys && a.k0 + a.lk < p.Tk;
+        if (x.twin) {
+          x.nt[1] = n / 2;
+          x.nt[0] = n - x.nt[1];
+        }
+        x.part = part;
+        x.valid = 1;
+        send(x);
+      };
+      // Works out the division of the last items: their work, lane by lane, and its prefix.
+      auto divide = [&]() {
+        if (!walk.find(p, whole, lane, a)) return;  // (none are left)
+        int work[kMaxShares / 32];
+#pragma unroll
+        for (int k = 0; k < kMaxShares / 32; ++k) work[k] = 0;
+        int base = 0, b = walk.block;
+        base = walk.base;
+        const int span = 2 * p.positions;
+        for (; b < p.batch && base < items; ++b) {
+          AttnPlace at;
+          attn_bounds(p.cu_q, b, p.Tq, at.q0, at.lq);
+          attn_bounds(p.cu_k, b, p.Tk, at.k0, at.lk);
+          const int n = (at.lq + span - 1) / span * p.heads_kv;
+#pragma unroll
+          for (int k = 0; k < kMaxShares / 32; ++k) {
+            const int x = whole + 32 * k + lane - base;
+            if (x >= 0 && x < n) {
+              attn_place(p, x, at);
+              work[k] = attn_work(p, at);
+            }
+          }
+          base += n;
+        }
+        int total = 0;
+        if (lane == 0) pre[0] = 0;
+#pragma unroll
+        for (int k = 0; k < kMaxShares / 32; ++k) {
+          int upto = work[k];
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+          }
+          if (32 * k + lane < sh.items) pre[32 * k + lane + 1] = total + upto;
+          total += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        __syncwarp();
+        sh.total = total;
+        // A share of less than 8 units costs more than it saves, unless it is an item of its own.  (No two edges can fall
+        // on one step: they are at least two units apart.)
+        sh.shares = max(1, min(p.shares, max(total / 8, min(sh.items, total / 2))));
+      };
+      int v = blockIdx.x;
+      while (v >= 0) {
+        if (v < whole) {
+          walk.find(p, v, lane, a);
+          send_steps(0, 0x7fffff, -1);
+        } else if (p.shares > 0 && v < whole + p.shares) {
+          const int s = v - whole;
+          if (sh.shares == 0) divide();
+          if (s == 0) {  // for the kernel that joins the parts
+            for (int x = lane; x <= sh.items; x += 32) p.meta[4 + x] = sh.items ? pre[x] : 0;
+            if (lane == 0) p.meta[0] = sh.shares, p.meta[1] = sh.items, p.meta[2] = whole;
+          }
+          if (s < sh.shares) {
+            auto edge = [&](int t) {
+              const int64_t x = static_cast<int64_t>(sh.total) * t / sh.shares;
+              if (t >= sh.shares) return sh.total;
+              const int i = sh.item_at(static_cast<int>(x), lane);
+              walk.find(p, whole + i, lane, a);
+              return sh.edge(t, attn_unit(p, a), i);
+            };
+            const int begin = edge(s), end = edge(s + 1);
+            for (int x = begin; x < end;) {
+              const int i = sh.item_at(x, lane);
+              walk.find(p, whole + i, lane, a);
+              const int unit = attn_unit(p, a), from = pre[i], upto = min(pre[i + 1], end);
+              const bool part = x > from || upto < pre[i + 1];
+              send_steps((x - from) / unit, (upto - from) / unit, part ? 2 * s + (x > from ? 0 : 1) : -1);
+              x = upto;
+            }
+          }
+        }
+        // The next one, once this one's loads are all under way (a few steps before its end): asked for earlier, it
+        // would be taken from CTAs that are free sooner.
+        if (sent > 0) guard.wait(want, (sent - 1) & 1);
+        const int slot = asked & 1;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bars + 2 * S + 18 + slot, 16);
+          launch_cancel(answers + 16 * slot, answer_full(slot));
+        }
+        __syncwarp();
+        guard.wait(answer_full(slot), (asked >> 1) & 1);
+        v = uniform(launch_cancelled(answers + 16 * slot));
+        fence_proxy_async_smem();  // the answer was read before it is overwritten
+        __syncwarp();
+        ++asked;
+        if (guard.aborted()) v = -1;
+      }
+      AttnItem end;
+      end.q_row = end.left = end.k_row = end.keys = end.head = end.see = end.nt[0] = end.nt[1] = 0;
+      end.twin = end.fixing = end.part = end.valid = 0;
+      send(end);
+    } else if (warp == 9) {
       // -------------------------------------------------------------- TMA producer
       uint32_t stage = 0, phase = 0, issued_mask = 0, issued_parity = 0;
       uint32_t q_count[2] = {0, 0};
       bool stop = false;
-      for (int item = blockIdx.x; !stop && walk.find(p, item, lane, it); item += gridDim.x) {
-        const int n0 = attn_tiles(p, it, 0), n1 = attn_tiles(p, it, 1);
-        const int n = max(n0, n1);
+      while (next_item()) {
+        copy_item();
         if (lane == 0) {
           auto load_q = [&](int i) {
             guard.wait(q_empty(i), (q_count[i] & 1) ^ 1);
-            if ((stop = *abort_flag != 0)) return;
+            if ((stop = guard.aborted())) return;
             uint64_t* full = bars + 2 * S + i;
             mbar_arrive_expect_tx(full, NP * 128 * p.positions * p.group);
             for (int c = 0; c < NP; ++c)
               tma_load_3d(q_smem + i * Cfg::kTileBytes + c * kAtPanelBytes, &tmap_q, full, c * 64, it.head * p.group,
-                          it.q0 + it.pos + i * p.positions);
+                          it.q_row + i * p.positions);
             ++q_count[i];
           };
           auto load_kv = [&](const CUtensorMap* map, int tile) {
+            if (stop) return;
             guard.wait(kv_empty(stage), phase ^ 1);
-            if ((stop = *abort_flag != 0)) return;
+            if ((stop = guard.aborted())) return;
             uint64_t* full = bars + stage;
             mbar_arrive_expect_tx(full, Cfg::kTileBytes);
             for (int c = 0; c < NP; ++c)
               tma_load_3d(ring + stage * Cfg::kTileBytes + c * kAtPanelBytes, map, full, c * 64, it.head,
-                          it.k0 + tile * kAtTile);
+                          it.k_row + tile * kAtTile);
             issued_mask |= 1u << stage;
             issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
             if (++stage == S) {
@@ -464,16 +714,28 @@ __global__ void __launch_bounds__(kAtThreads, 1)
               phase ^= 1;
             }
           };
-          if (n0 > 0) load_q(0);
-          for (int j = 0; !stop && j < n; ++j) {
-            load_kv(&tmap_k, it.t_lo + j);
-            if (!stop && j == 0 && n1 > 0) load_q(1);
-            if (!stop) load_kv(&tmap_v, it.t_lo + j);
+          if (it.nt[0] > 0) load_q(0);
+          if (it.twin) {  // K0 K1 | V0 K2 V1 K3 | V2 ...
+            const int n = it.nt[0] + it.nt[1];
+            load_kv(&tmap_k, 0);
+            load_kv(&tmap_k, 1);
+            for (int t = 0; !stop && t < n; ++t) {
+              load_kv(&tmap_v, t);
+              if (t + 2 < n) load_kv(&tmap_k, t + 2);
+            }
+          } else {  // K0 V0 | K1 V1 | ...
+            const int n = max(it.nt[0], it.nt[1]);
+            for (int j = 0; !stop && j < n; ++j) {
+              load_kv(&tmap_k, j);
+              if (!stop && j == 0 && it.nt[1] > 0) load_q(1);
+              load_kv(&tmap_v, j);
+            }
           }
+          bar_arrive(want);
         }
-        stop = uniform(stop ? 1 : 0) != 0;
+        __syncwarp();
       }
-      if (stop && lane == 0) {  // let every load this thread issued land before the CTA leaves
+      if (guard.aborted() && lane == 0) {  // let every load this thread issued land before the CTA leaves
         volatile int never = 0;
         for (int s = 0; s < S; ++s)
           if (issued_mask >> s & 1) mbar_wait_bounded(bars + s, issued_parity >> s & 1, p.wait_limit_ns, &never);
@@ -502,8 +764,8 @@ __global__ void __launch_bounds__(kAtThreads, 1)
           slot_phase ^= 1;
         }
       };
-      auto qk = [&](int i, uint32_t s) {  // S_i = Q_i K^T, by the elected lane
-        const uint64_t a0 = q_desc + i * kTileStep, b0 = k_desc + s * kTileStep;
+      auto qk = [&](int i, uint32_t q, uint32_t s) {  // S_i = Q K^T, by the elected lane
+        const uint64_t a0 = q_desc + q * kTileStep, b0 = k_desc + s * kTileStep;
 #pragma unroll
         for (int k = 0; k < 4 * NP; ++k) {
           const uint32_t off = ((k >> 2) * kAtPanelBytes + (k & 3) * 32) >> 4;
@@ -511,50 +773,56 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         }
         bar_commit(s_full(i));
       };
-      for (int item = blockIdx.x; walk.find(p, item, lane, it); item += gridDim.x) {
-        const int nt[2] = {uniform(attn_tiles(p, it, 0)), uniform(attn_tiles(p, it, 1))};
-        const int n = max(nt[0], nt[1]);
+      while (next_item()) {
+        copy_item();
+        const bool twin = it.twin != 0;
+        const int n = max(it.nt[0], it.nt[1]), all = it.nt[0] + it.nt[1];
         if (n == 0) continue;
         uint32_t ks = 0, kph = 0, vs = 0, vph = 0;
-        take(ks, kph);
-        guard.wait(kv_full(ks), kph);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (nt[i] > 0) {
+          if (i == 0 || twin) {
+            take(ks, kph);
+            guard.wait(kv_full(ks), kph);
+          }
+          if (it.nt[i] > 0 && !(i == 1 && twin)) {
             guard.wait(q_full(i), q_count[i] & 1);
             ++q_count[i];
           }
           tc_fence_after();
           if (elect_one()) {
-            if (nt[i] > 0) qk(i, ks);
-            if (nt[i] == 1) bar_commit(q_empty(i));
-            if (i == 1) bar_commit(kv_empty(ks));
+            if (it.nt[i] > 0) qk(i, twin ? 0 : i, ks);
+            if (twin ? all == 2 && i == 1 : it.nt[i] == 1) bar_commit(q_empty(twin ? 0 : i));
+            if (i == 1 || twin) bar_commit(kv_empty(ks));
           }
           __syncwarp();
         }
         for (int j = 0; j < n; ++j) {
-          take(vs, vph);
-          if (j + 1 < n) {  // (the loads run ahead: neither wait lasts)
-            take(ks, kph);
-            guard.both(kv_full(vs), vph, kv_full(ks), kph);
-          } else {
-            guard.wait(kv_full(vs), vph);
-          }
-          // cleared by warp 10 while the softmax still works on this tile
-          bool fixing = uniform((it.t_lo + j + 1) * kAtTile > it.lk && it.k0 + it.lk < p.Tk);
-          if (fixing && lane == 0) bar_arrive(v_need);
-          const uint64_t b0 = v_desc + vs * kTileStep;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t d = tmem + Cfg::kO + i * (NP * 64), a0 = tmem + i * 128;
-            const bool works = j < nt[i], ends = j + 1 == nt[i];
-            if (works) {
-              guard.wait(p_full(i, 0), p_count[i] & 1);
-              if (fixing) {
+            const bool works = j < it.nt[i], ends = j + 1 >= it.nt[i];
+            if (twin && !works) continue;
+            const int tile = twin ? 2 * j + i : j;  // key tile whose weights are multiplied
+            const bool has_k = twin ? tile + 2 < all : j + 1 < n;
+            if (i == 0 || twin) {
+              take(vs, vph);
+              if (has_k) {  // (the loads run ahead: neither wait lasts)
+                take(ks, kph);
+                guard.both(kv_full(vs), vph, kv_full(ks), kph);
+              } else {
+                guard.wait(kv_full(vs), vph);
+              }
+              // cleared by warp 10 while the softmax still works on this tile
+              if (it.fixing && tile + 1 == (twin ? all : n)) {
+                if (lane == 0) bar_arrive(v_need);
                 guard.wait(v_fixed, fixes & 1);
-                fixing = false;
                 ++fixes;
               }
+            }
+            const uint64_t b0 = v_desc + vs * kTileStep;
+            const uint32_t d = tmem + Cfg::kO + i * 128, a0 = tmem + i * 128;
+            if (works) {
+              guard.wait(p_full(i, 0), p_count[i] & 1);
               tc_fence_after();
               if (elect_one()) {
 #pragma unroll
@@ -574,20 +842,20 @@ __global__ void __launch_bounds__(kAtThreads, 1)
                 if (ends) {
                   bar_commit(o_full(i));
                 } else {
-                  qk(i, ks);
-                  if (j + 2 == nt[i]) bar_commit(q_empty(i));
+                  qk(i, twin ? 0 : i, ks);
+                  if (twin ? tile + 3 == all : j + 2 == it.nt[i]) bar_commit(q_empty(twin ? 0 : i));
                 }
               }
-              if (i == 1) {  // both tiles are served
+              if (i == 1 || twin) {  // all that read the slots are issued
                 bar_commit(kv_empty(vs));
-                if (j + 1 < n) bar_commit(kv_empty(ks));
+                if (has_k) bar_commit(kv_empty(ks));
               }
             }
             __syncwarp();
           }
         }
       }
-      if (*abort_flag) {  // the products still in flight read shared memory and TMEM
+      if (guard.aborted()) {  // the products still in flight read shared memory and TMEM
         volatile int never = 0;
         if (elect_one()) bar_commit(drain);
         __syncwarp();
@@ -598,13 +866,14 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       // Their weights are exactly zero, but 0 * NaN is not: another request's rows must not reach this one.  (Rows
       // behind the tensor's end are zeros that TMA filled in.)
       uint32_t slot = 0, fixes = 0;
-      for (int item = blockIdx.x; walk.find(p, item, lane, it); item += gridDim.x) {
-        const int n = max(attn_tiles(p, it, 0), attn_tiles(p, it, 1));
+      while (next_item()) {
+        copy_item();
+        const int n = it.twin ? it.nt[0] + it.nt[1] : max(it.nt[0], it.nt[1]);
         if (n == 0) continue;
-        const int rows = it.lk - (it.t_lo + n - 1) * kAtTile;
-        const uint32_t at = (slot + 2 * n - 1) % S;  // the item's last value tile
+        const uint32_t at = (slot + 2 * n - 1) % S;  // the last value tile is the item's last load
         slot = (slot + 2 * n) % S;
-        if (rows >= kAtTile || it.k0 + it.lk >= p.Tk) continue;
+        if (!it.fixing) continue;
+        const int rows = it.keys - (n - 1) * kAtTile;
         guard.wait(v_need, fixes & 1);
         ++fixes;
         __syncwarp();
@@ -619,26 +888,32 @@ __global__ void __launch_bounds__(kAtThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- softmax and output of tile i
-    setmaxnreg_inc<216>();
+    setmaxnreg_inc<224>();
     const int i = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + i * 128;
-    const uint32_t o_addr = tmem + lanes + Cfg::kO + i * (NP * 64);
-    const int row_pos = row / p.group, row_head = row - row_pos * p.group;
+    const uint32_t s_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + i * 128;
     const float c2 = p.scale_log2;
-    uint32_t count = 0, items = 0;
-    for (int item = blockIdx.x; walk.find(p, item, lane, it); item += gridDim.x) {
-      const int n = uniform(attn_tiles(p, it, i));
-      const int pos = it.pos + i * p.positions + row_pos;
-      const bool valid = row_pos < p.positions && pos < it.lq;
-      const int keys = !valid ? 0 : (p.causal ? min(it.lk, pos + it.lk - it.lq + 1) : it.lk);
+    uint32_t s_phase = 0, o_phase = 0, twin_phase = 0;
+    while (next_item()) {
+      const bool twin = uniform(item->twin) != 0;
+      const int n = uniform(item->nt[i]);
+      // (registers are short below: what only the output needs is worked out again there)
+      auto position = [&](bool& valid) {
+        const int in_tile = row / p.group;
+        const int pos = (twin ? 0 : i * p.positions) + in_tile;
+        valid = in_tile < p.positions && pos < item->left;
+        return pos;
+      };
+      bool valid;
+      const int pos = position(valid);
+      const int keys = !valid ? 0 : (p.causal ? min(item->keys, item->see + pos) : item->keys);
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       // tiles before this one need no mask in any row of the warp
       const int full = __reduce_min_sync(0xffffffffu, valid ? max(keys, 0) : 0x7fffffff) / kAtTile;
       float m = -CUDART_INF_F, l = 0.0f;
-      for (int j = 0; j < n; ++j, ++count) {
-        guard.poll(s_full(i), count & 1);
+      for (int j = 0; j < n; ++j) {
+        guard.poll(s_full(i), s_phase);
+        s_phase ^= 1;
         __syncwarp();
         auto hand_over = [&](int part) {
           tmem_st_wait();
@@ -652,12 +927,13 @@ __global__ void __launch_bounds__(kAtThreads, 1)
           continue;
         }
         tc_fence_after();
+        const int tile = twin ? 2 * j + i : j;
         uint32_t s[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
         tmem_ld_wait();
-        if (it.t_lo + j >= full) {
-          const int seen = keys - (it.t_lo + j) * kAtTile;
+        if (tile >= full) {
+          const int seen = keys - tile * kAtTile;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -695,11 +971,11 @@ __global__ void __launch_bounds__(kAtThreads, 1)
 #pragma unroll 1
             for (int c = 0; c < 2 * NP; ++c) {
               uint32_t o[32];
-              tmem_ld_32x32b_x32(o_addr + c * 32, o);
+              tmem_ld_32x32b_x32(s_addr + Cfg::kO + c * 32, o);
               tmem_ld_wait();
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st_32x32b_x32(o_addr + c * 32, o);
+              tmem_st_32x32b_x32(s_addr + Cfg::kO + c * 32, o);
             }
           }
         }
@@ -717,56 +993,105 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       }
       // ------------------------------------------------------------ the item's rows
       if (n > 0) {
-        guard.wait(o_full(i), items & 1);
-        ++items;
+        guard.wait(o_full(i), o_phase);
+        o_phase ^= 1;
         __syncwarp();
         tc_fence_after();
       }
-      if (!warp_valid) continue;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees no key gives zeros
-      const int64_t t = it.q0 + pos;
-      const int head = it.head * p.group + row_head;
-      const int heads = p.heads_kv * p.group;
-      const bool parts = p.max_splits > 1;
-      const int64_t part = ((static_cast<int64_t>(it.split) * p.Tq + t) * heads + head);
-#pragma unroll
-      for (int c = 0; c < 2 * NP; ++c) {
-        uint32_t o[32];
-        if (n > 0) {
-          tmem_ld_32x32b_x32(o_addr + c * 32, o);
-          tmem_ld_wait();
+      float w0 = 1.0f, w1 = 0.0f;  // of this tile's o, and of tile 1's in a twin item
+      if (twin) {
+        if (i == 1) {  // m and l go where the scores were
+          tmem_st_32x32b_x2(s_addr, __float_as_uint(m), __float_as_uint(l));
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(twin_ready);
+          guard.wait(twin_done, twin_phase);
+          twin_phase ^= 1;
+          release();
+          continue;
         }
-        if (valid) {
+        guard.wait(twin_ready, twin_phase);
+        twin_phase ^= 1;
+        __syncwarp();
+        tc_fence_after();
+        uint32_t a, b;
+        tmem_ld_32x32b_x2(s_addr + 128, a, b);
+        tmem_ld_wait();
+        const float m1 = __uint_as_float(a), l1 = __uint_as_float(b);
+        const float top = max3(m, m1, m1);  // NaN if one is
+        if (top != -CUDART_INF_F) {
+          w0 = m == -CUDART_INF_F ? 0.0f : exp2_approx((m - top) * c2);
+          w1 = m1 == -CUDART_INF_F ? 0.0f : exp2_approx((m1 - top) * c2);
+          l = l * w0 + l1 * w1;
+          m = top;
+        }
+      }
+      if (warp_valid) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees no key gives zeros
+        w0 *= inv;
+        w1 *= inv;
+        const bool parts = uniform(item->part) >= 0, any = n > 0 && inv != 0.0f;
+        int r = row;
+        asm volatile("" : "+r"(r));  // not kept from before
+        const int in_tile = r / p.group;
+        const int64_t t = item->q_row + (twin ? 0 : i * p.positions) + in_tile;
+        const int head = item->head * p.group + r - in_tile * p.group;
+        const int64_t part = static_cast<int64_t>(item->part) * 256 + i * 128 + row;
+#pragma unroll 1
+        for (int c = 0; c < 2 * NP; ++c) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_ld_32x32b_x32(s_addr + Cfg::kO + c * 32, o);
+            tmem_ld_wait();
+          }
+          if (twin) {
+            uint32_t o1[32];
+            tmem_ld_32x32b_x32(s_addr + Cfg::kO + 128 + c * 32, o1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), w1, __uint_as_float(o[e]) * w0));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0);
+          }
+          if (!valid) continue;
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             const int col = c * 32 + e;
-            if (col < p.D) {
-              float f[8];
+            if (col >= p.D) continue;
+            float f[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) f[k] = n > 0 && inv != 0.0f ? __uint_as_float(o[e + k]) * inv : 0.0f;
-              if (parts) {
-                float4* dst = reinterpret_cast<float4*>(p.part_o + part * p.D + col);
-                dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-                dst[1] = make_float4(f[4], f[5], f[6], f[7]);
-              } else {
-                uint4 u;
-                u.x = Pack16<T>::pack(f[0], f[1]);
-                u.y = Pack16<T>::pack(f[2], f[3]);
-                u.z = Pack16<T>::pack(f[4], f[5]);
-                u.w = Pack16<T>::pack(f[6], f[7]);
-                *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_t + head * p.out_h + col) = u;
-              }
+            for (int k = 0; k < 8; ++k) f[k] = any ? __uint_as_float(o[e + k]) : 0.0f;
+            if (parts) {
+              float4* dst = reinterpret_cast<float4*>(p.part_o + part * p.D + col);
+              dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+              dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+            } else {
+              uint4 u;
+              u.x = Pack16<T>::pack(f[0], f[1]);
+              u.y = Pack16<T>::pack(f[2], f[3]);
+              u.z = Pack16<T>::pack(f[4], f[5]);
+              u.w = Pack16<T>::pack(f[6], f[7]);
+              *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_t + head * p.out_h + col) = u;
             }
           }
         }
+        if (valid) {
+          const float lse2 = l == 0.0f ? -CUDART_INF_F : fmaf(m, c2, log2f(l));
+          if (parts)
+            p.part_lse[part] = lse2;
+          else if (p.lse)
+            p.lse[t * (p.heads_kv * p.group) + head] = lse2 * 0.69314718055994530942f;
+        }
       }
-      if (valid) {
-        const float lse2 = l == 0.0f ? -CUDART_INF_F : fmaf(m, c2, log2f(l));
-        if (parts)
-          p.part_lse[part] = lse2;
-        else if (p.lse)
-          p.lse[t * heads + head] = lse2 * 0.69314718055994530942f;
+      if (twin) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(twin_done);
       }
+      release();
     }
   }
 
@@ -778,54 +1103,71 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   }
 }
 
-// Joins the key splits: o = sum_s w_s o_s with w_s = 2^(lse_s - m) / sum 2^(lse_s - m), in split order.  One warp for
-// each row of out; the partial rows were just written and mostly come from L2.
+// Joins the parts of the items that were divided: o = sum_s w_s o_s with w_s = 2^(lse_s - m) / sum 2^(lse_s - m), in the
+// order of the shares.  Block (x, y): rows y, y + gridDim.y, ... (by eights) of the x-th divided item; one warp a row.  The
+// partial rows were just written and mostly come from L2.
 template <class T>
 __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_constant__ AttnParams p) {
-  const int heads = p.heads_kv * p.group;
   const int lane = threadIdx.x & 31;
-  const int64_t rows = static_cast<int64_t>(p.Tq) * heads;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (r >= rows) return;
-  const int t = static_cast<int>(r / heads);
-  const int head = static_cast<int>(r - static_cast<int64_t>(t) * heads);
-  int q0 = 0, lq = p.Tq, k0 = 0, lk = p.Tk;
-  if (p.cu_q) {  // the last sequence that starts at or before t (offsets do not decrease)
-    int lo = 0, hi = p.batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(p.cu_q + mid) <= t)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    attn_bounds(p.cu_q, lo, p.Tq, q0, lq);
-    attn_bounds(p.cu_k, lo, p.Tk, k0, lk);
-    if (t < q0 || t >= q0 + lq) return;  // a row of no sequence stays as it was
+  const int shares = p.meta[0], items = p.meta[1], whole = p.meta[2], x = blockIdx.x;
+  // (the limits also hold if the first kernel gave up and left no plan)
+  if (x >= items || items >= kMaxShares || shares < 1 || shares > p.shares) return;
+  const int* pre = p.meta + 4;
+  const AttnShares sh{pre, items, pre[items], shares};
+  const int from = pre[x], upto = pre[x + 1];
+  AttnWalk walk;
+  AttnPlace a;
+  if (!walk.find(p, whole + x, lane, a)) return;
+  const int unit = attn_unit(p, a);
+  // the edges that lie inside this item
+  int s = max(1, static_cast<int>((static_cast<int64_t>(from) * shares + sh.total - 1) / max(sh.total, 1)));
+  int first = 0, last = -1;  // shares of the item, if it was divided
+  for (; s < shares && static_cast<int64_t>(sh.total) * s / shares < upto; ++s) {
+    const int e = sh.edge(s, unit, x);
+    if (e <= from || e >= upto) continue;
+    if (last < 0) first = s - 1;
+    last = s;
   }
-  const int ns = attn_splits(p, lk);
-  float m = -CUDART_INF_F;
-  for (int s = lane; s < ns; s += 32) m = fmaxf(m, p.part_lse[s * rows + r]);
+  if (last < 0) return;
+  const int heads = p.heads_kv * p.group;
+  const int rows = min(a.lq - a.pos, 2 * p.positions) * p.group;
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
+    const int position = r / p.group, head = r - position * p.group;
+    const int tile = position >= p.positions ? 1 : 0;
+    const int at = tile * 128 + (position - tile * p.positions) * p.group + head;
+    auto slot = [&](int s) {  // the first part of an item is its share's last
+      return (2 * static_cast<int64_t>(s) + (s == first ? 1 : 0)) * 256 + at;
+    };
+    float m = -CUDART_INF_F;
+    for (int s = first + lane; s <= last; s += 32) m = max3(m, p.part_lse[slot(s)], p.part_lse[slot(s)]);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const int c = lane * 4;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float total = 0.0f;
-  for (int s = 0; s < ns; ++s) {
-    const float z = p.part_lse[s * rows + r];
-    if (z == -CUDART_INF_F) continue;
-    const float w = exp2f(z - m);
-    total += w;
-    if (c < p.D) {
-      const float4 f = *reinterpret_cast<const float4*>(p.part_o + (s * rows + r) * p.D + c);
-      acc.x = fmaf(w, f.x, acc.x), acc.y = fmaf(w, f.y, acc.y), acc.z = fmaf(w, f.z, acc.z), acc.w = fmaf(w, f.w, acc.w);
+    for (int o = 16; o; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, m, o);
+      m = max3(m, other, other);
     }
+    const int c = lane * 4;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float total = 0.0f;
+    for (int s = first; s <= last; ++s) {
+      const float z = p.part_lse[slot(s)];
+      if (z == -CUDART_INF_F) continue;
+      const float w = exp2f(z - m);
+      total += w;
+      if (c < p.D) {
+        const float4 f = *reinterpret_cast<const float4*>(p.part_o + slot(s) * p.D + c);
+        acc.x = fmaf(w, f.x, acc.x), acc.y = fmaf(w, f.y, acc.y);
+        acc.z = fmaf(w, f.z, acc.z), acc.w = fmaf(w, f.w, acc.w);
+      }
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const int64_t t = a.q0 + a.pos + position;
+    const int h = a.head * p.group + head;
+    if (c < p.D)
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.out_t + h * p.out_h + c) =
+          make_uint2(Pack16<T>::pack(acc.x * inv, acc.y * inv), Pack16<T>::pack(acc.z * inv, acc.w * inv));
+    if (p.lse && lane == 0)
+      p.lse[t * heads + h] = total == 0.0f ? -CUDART_INF_F : (m + log2f(total)) * 0.69314718055994530942f;
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  if (c < p.D)
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.out_t + head * p.out_h + c) =
-        make_uint2(Pack16<T>::pack(acc.x * inv, acc.y * inv), Pack16<T>::pack(acc.z * inv, acc.w * inv));
-  if (p.lse && lane == 0) p.lse[r] = total == 0.0f ? -CUDART_INF_F : (m + log2f(total)) * 0.69314718055994530942f;
 }
 
 }  // namespace convrot

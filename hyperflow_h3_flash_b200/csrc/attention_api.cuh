@@ -120,29 +120,24 @@ int attn_check(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv,
   return CONVROT_OK;
 }
 
-// How keys are split, from host-known sizes alone.
-void attn_plan(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int D, int sms, int* max_splits,
-               int* chunk_tiles) {
-  *max_splits = 1;
-  *chunk_tiles = 1;
-  if (batch < 1 || Tq < 1 || Tk < 1) return;
-  const int64_t positions = kAtTile / (heads_q / heads_kv);
-  const int64_t span = 2 * positions;
-  const int64_t q_tiles = batch > (Tq + span - 1) / span ? batch : (Tq + span - 1) / span;
-  const int64_t items = q_tiles * heads_kv;
-  const int64_t k_tiles = (Tk + kAtTile - 1) / kAtTile;  // of all sequences; one may hold them all
-  const int64_t mean = (k_tiles + batch - 1) / batch;
-  if (items >= 3 * sms && Tq > 4 * batch) return;
-  int64_t chunk = (items * mean + 4 * sms - 1) / (4 * sms);
-  if (chunk < 4) chunk = 4;
-  int64_t splits = (k_tiles + chunk - 1) / chunk;
-  const int64_t bytes = Tq * heads_q * (D + 1) * 4;
-  const int64_t most = (int64_t{96} << 20) / bytes;
-  if (splits > most) splits = most;
-  if (splits > 64) splits = 64;
-  if (splits <= 1) return;
-  *max_splits = static_cast<int>(splits);
-  *chunk_tiles = static_cast<int>(chunk);
+// Query tiles that a call has at most, from host-known sizes.
+int64_t attn_items(int64_t Tq, int64_t batch, int heads_q, int heads_kv) {
+  const int64_t span = 2 * (kAtTile / (heads_q / heads_kv));
+  const int64_t q_tiles = batch == 1 ? (Tq + span - 1) / span : Tq / span + (batch < Tq ? batch : Tq);
+  return q_tiles * heads_kv;
+}
+
+// CTAs that share the items of the last wave evenly; 0: every item is one CTA's.  Dividing costs a second launch and
+// the partial rows' way through memory (together about as long as four steps of two tiles); an uneven last wave costs up
+// to one item's time.  So not where items are short, nor where there are so many waves that the last hardly counts.
+int attn_shares(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int sms) {
+  if (batch < 1 || Tq < 1 || Tk < 8 * kAtTile) return 0;
+  const int shares = sms < kMaxShares ? sms : kMaxShares;
+  return attn_items(Tq, batch, heads_q, heads_kv) < 24 * static_cast<int64_t>(shares) ? shares : 0;
+}
+
+size_t attn_workspace(int shares, int D) {
+  return shares ? (kMaxShares + 4 + static_cast<size_t>(shares) * 2 * 256 * (D + 1)) * 4 : 0;
 }
 
 int attn_map(CUtensorMap* map, const void* base, int dtype, int D, int64_t heads, int64_t rows, int64_t ld_h,
@@ -175,12 +170,10 @@ int launch_attention(const DeviceState& st, const CUtensorMap& tq, const CUtenso
     if (e != cudaSuccess) return cuda_fail(e);
     store_resident(reinterpret_cast<const void*>(kernel), 1);
   }
-  const unsigned grid = static_cast<unsigned>(items < st.sms ? items : st.sms);
-  kernel<<<grid, kAtThreads, AttnCfg<NP>::kSmemBytes, stream>>>(tq, tk, tv, p);
+  kernel<<<static_cast<unsigned>(items), kAtThreads, AttnCfg<NP>::kSmemBytes, stream>>>(tq, tk, tv, p);
   if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e);
-  if (p.max_splits > 1) {
-    const int64_t rows = static_cast<int64_t>(p.Tq) * p.heads_kv * p.group;
-    attention_combine_kernel<T><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(p);
+  if (p.shares > 0) {
+    attention_combine_kernel<T><<<dim3(p.shares, 4), 256, 0, stream>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e);
   }
   return CONVROT_OK;
@@ -212,13 +205,13 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
   if ((rc = device_state(&st))) return rc;
   AttnParams p;
   memset(&p, 0, sizeof(p));
-  attn_plan(Tq, Tk, batch, heads_q, heads_kv, D, st->sms, &p.max_splits, &p.chunk_tiles);
-  if (p.max_splits > 1) {
-    const size_t rows = static_cast<size_t>(p.max_splits) * Tq * heads_q;
-    if (!workspace || workspace_bytes < rows * (D + 1) * 4) return CONVROT_ERR_ARG;
+  p.shares = attn_shares(Tq, Tk, batch, heads_q, heads_kv, st->sms);
+  if (p.shares > 0) {
+    if (!workspace || workspace_bytes < attn_workspace(p.shares, D)) return CONVROT_ERR_ARG;
     if (!aligned16(workspace)) return CONVROT_ERR_ALIGN;
-    p.part_o = static_cast<float*>(workspace);
-    p.part_lse = p.part_o + rows * D;
+    p.meta = static_cast<int*>(workspace);
+    p.part_o = static_cast<float*>(workspace) + kMaxShares + 4;
+    p.part_lse = p.part_o + static_cast<size_t>(p.shares) * 2 * 256 * D;
   }
   p.cu_q = cu_q;
   p.cu_k = cu_k;
@@ -246,10 +239,9 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
   if ((rc = attn_map(&tv, Tk ? v : q, dtype, D, Tk ? heads_kv : heads_q, Tk ? Tk : Tq, Tk ? v_h : q_h, Tk ? v_t : q_t, 1,
                      kAtTile)))
     return rc;
-  // An upper bound of the work items (the kernel finds their number): every CTA beyond it would find nothing.
-  const int64_t span = 2 * p.positions;
-  const int64_t q_tiles = batch == 1 ? (Tq + span - 1) / span : Tq / span + (batch < Tq ? batch : Tq);
-  const int64_t items = q_tiles * heads_kv * p.max_splits;
+  // An upper bound of the work items (the kernel finds their number; what is beyond it finds nothing).
+  const int64_t items = attn_items(Tq, batch, heads_q, heads_kv) + p.shares;
+  if (items > INT32_MAX / 2) return CONVROT_ERR_SHAPE;
   if (dtype == 0)
     return D <= 64 ? launch_attention<__nv_bfloat16, 1>(*st, tq, tk, tv, p, items, stream)
                    : launch_attention<__nv_bfloat16, 2>(*st, tq, tk, tv, p, items, stream);
