@@ -34,20 +34,21 @@ MAX_HEAD_DIM = 128  # of attention; qk_norm_rope takes heads up to 256
 
 
 def _no_grad(*tensors: Tensor | None) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("attention operators are inference only: use torch.no_grad() or detach the inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError("attention operators are inference only: use torch.no_grad() or detach the inputs")
 
 
 def _call(fn: str, device: torch.device, *args) -> None:
     """One library call on the tensors' device and its current stream."""
-    handle = _lib.lib()
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            rc = getattr(handle, fn)(*args, torch.cuda.current_stream(device).cuda_stream)
+    # (the raw stream of the allocator's bookkeeping: a torch.cuda.Stream object takes longer to make than the launch)
+    index = device.index
+    entry = getattr(_lib.lib(), fn)
+    if index == torch._C._cuda_getDevice():
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        rc = getattr(handle, fn)(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(device):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, fn)
 
@@ -61,6 +62,10 @@ def _heads(t: Tensor, name: str, like: Tensor | None = None) -> None:
         raise ValueError(f"{name} must be contiguous in its last dimension")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+
+
+def _new(x: Tensor) -> Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 # ------------------------------------------------------------------------------------------------ positions
@@ -128,7 +133,7 @@ def _norm_rope_torch(x: Tensor, weight: Tensor | None, eps: float, norm: bool, t
 
 def _rope_out(out: Tensor | None, x: Tensor, name: str) -> Tensor:
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return _new(x)
     _heads(out, name, x)
     if out.shape != x.shape:
         raise ValueError(f"{name} must have shape {tuple(x.shape)}, got {tuple(out.shape)}")
@@ -145,7 +150,8 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
     (``rotary_table``'s, fp32 ``[T, R / 2, 2]``; None: no rotation): pairs of neighbours if ``interleaved``, else
     ``(j, j + R / 2)``.  fp32 arithmetic, one rounding.  Returns the new q (and k when given).  ``q_out`` / ``k_out`` may
     be the inputs themselves; an output that overlaps an input in any other way is not supported."""
-    _no_grad(q, k, q_weight, k_weight)
+    if torch.is_grad_enabled():
+        _no_grad(q, k, q_weight, k_weight)
     _heads(q, "q")
     if k is not None:
         _heads(k, "k", q)
@@ -153,7 +159,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
             raise ValueError(f"k must have q's tokens and head_dim, got {tuple(k.shape)} beside {tuple(q.shape)}")
     elif k_weight is not None or k_out is not None:
         raise ValueError("k_weight and k_out need k")
-    T, D = q.shape[0], q.shape[2]
+    T, _, D = q.shape
     if not norm and table is None:
         raise ValueError("nothing to do: norm=False and no table")
     if not norm and (q_weight is not None or k_weight is not None):
@@ -193,13 +199,16 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
         raise ValueError("q_out and k_out must not be the other's input or each other")
     if q.shape[1] == 0 or (k is not None and k.shape[1] == 0):
         raise ValueError("q and k need at least one head")
-    kk = (None, 0, 0, None, 0, 0, 0) if k is None else (k.data_ptr(), k.stride(0), k.stride(1), ko.data_ptr(),
-                                                        ko.stride(0), ko.stride(1), k.shape[1])
-    _call("convrot_qk_norm_rope", q.device, q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0),
-          qo.stride(1), q.shape[1], *kk, T, D, _DTYPES[q.dtype], norm,
-          None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-          bool(weights) and weights[0].dtype == torch.float32, eps, None if table is None else table.data_ptr(), R // 2,
-          R, interleaved)
+    qs, qos = q.stride(), qo.stride()
+    if k is None:
+        kk = (None, 0, 0, None, 0, 0, 0)
+    else:
+        ks, kos = k.stride(), ko.stride()
+        kk = (k.data_ptr(), ks[0], ks[1], ko.data_ptr(), kos[0], kos[1], k.shape[1])
+    _call("convrot_qk_norm_rope", q.device, q.data_ptr(), qs[0], qs[1], qo.data_ptr(), qos[0], qos[1], q.shape[1], *kk, T,
+          D, _DTYPES[q.dtype], norm, None if q_weight is None else q_weight.data_ptr(),
+          None if k_weight is None else k_weight.data_ptr(), bool(weights) and weights[0].dtype == torch.float32, eps,
+          None if table is None else table.data_ptr(), R // 2, R, interleaved)
     return qo if k is None else (qo, ko)
 
 
@@ -242,7 +251,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
 
     Scores, statistics and sums are fp32; the weights are rounded to the inputs' type for their product with v.  Few
     queries over long keys are split over the GPU and joined in a fixed order: results do not vary from run to run."""
-    _no_grad(q, k, v)
+    if torch.is_grad_enabled():
+        _no_grad(q, k, v)
     _heads(q, "q")
     _heads(k, "k", q)
     _heads(v, "v", q)
@@ -269,7 +279,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
             raise ValueError(f"cu_q and cu_k must have one length, got {cu_q.shape[0]} and {cu_k.shape[0]}")
         batch = cu_q.shape[0] - 1
     if out is None:
-        out = torch.empty(Tq, Hq, D, dtype=q.dtype, device=q.device)
+        out = _new(q)
     else:
         _heads(out, "out", q)
         if out.shape != q.shape:
@@ -278,19 +288,20 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
     if not q.is_cuda:
         _attention_torch(q, k, v, cu_q, cu_k, causal, scale, out, lse)
         return out if lse is None else (out, lse)
-    if q.device.index != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
-            size = _lib.lib().convrot_attention_workspace_size(Tq, Tk, batch, Hq, Hkv, D)
+    handle, device = _lib.lib(), q.device
+    if device.index == torch._C._cuda_getDevice():
+        size = handle.convrot_attention_workspace_size(Tq, Tk, batch, Hq, Hkv, D)
     else:
-        size = _lib.lib().convrot_attention_workspace_size(Tq, Tk, batch, Hq, Hkv, D)
+        with torch.cuda.device(device):
+            size = handle.convrot_attention_workspace_size(Tq, Tk, batch, Hq, Hkv, D)
     if size < 0:
         raise ValueError(f"attention does not take {Tq} queries and {Tk} keys in {batch} sequences of {Hq} heads")
     # from torch's stream-ordered allocator: freed at return, reused only by later work of this stream (or graph)
-    space = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    _call("convrot_attention", q.device, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-          v.data_ptr(), v.stride(0), v.stride(1), None if cu_q is None else cu_q.data_ptr(),
-          None if cu_k is None else cu_k.data_ptr(), batch, Tq, Tk, Hq, Hkv, D, _DTYPES[q.dtype], scale, causal,
-          out.data_ptr(), out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(),
+    space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    _call("convrot_attention", device, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+          None if cu_q is None else cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(), batch, Tq, Tk, Hq, Hkv, D,
+          _DTYPES[q.dtype], scale, causal, out.data_ptr(), os[0], os[1], None if lse is None else lse.data_ptr(),
           None if space is None else space.data_ptr(), size)
     return out if lse is None else (out, lse)
 

@@ -84,23 +84,28 @@ int qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t q
   p.rows = rows;
   p.D = D;
   p.R = table ? R : 0;
-  while ((8 << p.lanes_log2) < D) ++p.lanes_log2;
-  const int per = kRopeRows * (32 >> p.lanes_log2);
-  p.items = (heads_q + heads_k + per - 1) / per;
+  // a lane holds 8 channels (pairs of neighbours), or 8 and their partners, or 16 behind the rotated part
+  const bool single = !table || interleaved;
+  const int lanes = single ? D / 8 : p.R / 16 + (D - p.R + 15) / 16;
+  while ((1 << p.lanes_log2) < lanes) ++p.lanes_log2;
+  const int per = (single ? kRopeRows : kRopeRows / 2) * (32 >> p.lanes_log2);
+  p.items_q = (heads_q + per - 1) / per;
+  p.items = p.items_q + (heads_k + per - 1) / per;
   p.norm = norm;
   p.weight_f32 = weight_f32;
   p.eps = eps;
+  p.inv_D = 1.0f / static_cast<float>(D);
   const int64_t blocks = (rows * p.items + kRopeWarps - 1) / kRopeWarps;
   if (blocks > INT32_MAX) return CONVROT_ERR_SHAPE;
   const unsigned grid = static_cast<unsigned>(blocks);
   const int threads = kRopeWarps * 32;
   if (dtype == 0) {
-    if (interleaved)
+    if (single)
       qk_norm_rope_kernel<__nv_bfloat16, true><<<grid, threads, 0, stream>>>(p);
     else
       qk_norm_rope_kernel<__nv_bfloat16, false><<<grid, threads, 0, stream>>>(p);
   } else {
-    if (interleaved)
+    if (single)
       qk_norm_rope_kernel<__half, true><<<grid, threads, 0, stream>>>(p);
     else
       qk_norm_rope_kernel<__half, false><<<grid, threads, 0, stream>>>(p);

@@ -38,14 +38,23 @@ struct RotaryTableParams {
 
 template <class Pos>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ RotaryTableParams p) {
+  // (read from the arguments directly, 32 frequencies of a warp are 32 accesses one after the other: 33 us instead of
+  // 5 for 32760 x 64 pairs)
+  __shared__ double freq[kRopeMaxPairs];
+  __shared__ int axis[kRopeMaxPairs];
+  if (threadIdx.x < p.pairs) {
+    freq[threadIdx.x] = p.freq_over_pi[threadIdx.x];
+    axis[threadIdx.x] = p.axis[threadIdx.x];
+  }
+  __syncthreads();
   const int64_t n = p.rows * p.pairs;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += step) {
     // 32-bit division wherever it fits (a 64-bit one costs several times as much)
     const int64_t t = n <= 0x7fffffff ? static_cast<uint32_t>(i) / static_cast<uint32_t>(p.pairs) : i / p.pairs;
     const int j = static_cast<int>(i - t * p.pairs);
-    const double pos = static_cast<double>(static_cast<const Pos*>(p.pos)[t * p.ld_pos + p.axis[j]]);
-    double x = pos * p.freq_over_pi[j];
+    const double pos = static_cast<double>(static_cast<const Pos*>(p.pos)[t * p.ld_pos + axis[j]]);
+    double x = pos * freq[j];
     x = fma(-2.0, rint(0.5 * x), x);
     const float h = static_cast<float>(x);
     const float l = static_cast<float>((x - static_cast<double>(h)) * 3.14159265358979323846);
@@ -65,14 +74,14 @@ struct QkRopeParams {
   int64_t ld_table;     // pairs
   int64_t rows;         // T
   int D, R;
-  int lanes_log2;  // lanes of one head row: the power of two that holds D / 8
-  int items;       // warp items of one token
+  int lanes_log2;  // lanes of one head row: a power of two
+  int items, items_q;  // warp items of one token, and of its q
   int norm, weight_f32;
-  float eps;
+  float eps, inv_D;
 };
 
-constexpr int kRopeRows = 4;
-constexpr int kRopeWarps = 8;
+constexpr int kRopeRows = 4;  // 16-byte loads of a lane in flight
+constexpr int kRopeWarps = 2;
 
 template <class T>
 struct Pack16;
@@ -118,105 +127,127 @@ __device__ __forceinline__ void load_weight8(const void* w, int f32, int c, floa
   }
 }
 
+template <class T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
+  const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Pack16<T>::unpack(v[i]);
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
+}
+
+// A warp item is a few steps of rows of q or of k of one token.  Weights and rotation are joined once for all of an item's
+// rows: with (a, b) a pair and a' = inv a, b' = inv b, out = (a' (wa c) - b' (wb s), b' (wb c) + a' (wa s)), so a row
+// costs two operations an element beside its sum of squares and the scale.  (Every row with its own weight and rotation
+// took 350 us for 32760 tokens x 2 x 40 heads of 128, bound by issue slots.)  With pairs of neighbours a lane holds 8
+// channels; with pairs R / 2 apart it holds the 8 channels and their partners, R / 2 further (by shuffles from the
+// partners' lane they cost 306 us instead of 248), and lanes behind the rotated part hold 16 channels in a row.
 template <class T, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __grid_constant__ QkRopeParams p) {
+  constexpr int CH = INTERLEAVED ? 1 : 2;  // 8-channel pieces of a lane
+  constexpr int kSteps = kRopeRows / CH;
+  constexpr int kPartner = INTERLEAVED ? 1 : 8;
   const int lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kRopeWarps + (threadIdx.x >> 5);
   if (item >= p.rows * p.items) return;  // whole warps
-  const int64_t t = item / p.items;
+  const int64_t t = p.rows * p.items <= 0x7fffffff
+                        ? static_cast<uint32_t>(item) / static_cast<uint32_t>(p.items)
+                        : item / p.items;
   const int lanes = 1 << p.lanes_log2;
   const int at = lane & (lanes - 1);
-  const int c = at * 8;  // this lane's first channel
-  const bool here = c < p.D;
-  const int per = 32 >> p.lanes_log2;  // rows of one step of the warp
-  const int row0 = static_cast<int>(item - t * p.items) * (kRopeRows * per) + (lane >> p.lanes_log2);
-  const int total = p.heads[0] + p.heads[1];
-
-  uint4 raw[kRopeRows];
-  int which[kRopeRows], head[kRopeRows];
-#pragma unroll
-  for (int r = 0; r < kRopeRows; ++r) {
-    const int row = row0 + r * per;
-    which[r] = row >= total ? -1 : (row >= p.heads[0] ? 1 : 0);
-    head[r] = which[r] == 1 ? row - p.heads[0] : row;
-    raw[r] = make_uint4(0, 0, 0, 0);
-    if (here && which[r] >= 0) {
-      const int w = which[r];
-      raw[r] = *reinterpret_cast<const uint4*>(static_cast<const T*>(w ? p.in[1] : p.in[0]) +
-                                               t * (w ? p.in_t[1] : p.in_t[0]) +
-                                               head[r] * (w ? p.in_h[1] : p.in_h[0]) + c);
-    }
-  }
-
-  // (cos, sin) of this lane's channels: 4 pairs of neighbours, or 8 pairs half the rotated width apart
-  constexpr int kPairs = INTERLEAVED ? 4 : 8;
-  float2 cs[kPairs];
   const int half = p.R >> 1;
-  const bool turns = p.table && c < p.R;
-  const bool second = !INTERLEAVED && c >= half;
-  if (turns) {
-    const float4* src = reinterpret_cast<const float4*>(p.table + t * p.ld_table +
-                                                        (INTERLEAVED ? c >> 1 : (second ? c - half : c)));
+  const bool turns = INTERLEAVED ? at * 8 < p.R : at * 8 < half;
+  const int c = INTERLEAVED || turns ? at * 8 : p.R + (at * 8 - half) * 2;  // this lane's first channel
+  const int apart = turns ? half : 8;                                       // and its second piece (CH == 2)
+  const int per = 32 >> p.lanes_log2;                                       // rows of one step of the warp
+  int group = static_cast<int>(item - t * p.items);
+  const bool is_k = group >= p.items_q;
+  if (is_k) group -= p.items_q;
+  const int heads = is_k ? p.heads[1] : p.heads[0];
+  const int row0 = group * (kSteps * per) + (lane >> p.lanes_log2);
+  const int64_t in_h = is_k ? p.in_h[1] : p.in_h[0], out_h = is_k ? p.out_h[1] : p.out_h[0];
+  const T* in = static_cast<const T*>(is_k ? p.in[1] : p.in[0]) + t * (is_k ? p.in_t[1] : p.in_t[0]) + row0 * in_h + c;
+  T* out = static_cast<T*>(is_k ? p.out[1] : p.out[0]) + t * (is_k ? p.out_t[1] : p.out_t[0]) + row0 * out_h + c;
+  bool here[CH];
 #pragma unroll
-    for (int i = 0; i < kPairs / 2; ++i) {
-      const float4 f = __ldg(src + i);
-      cs[2 * i] = make_float2(f.x, f.y);
-      cs[2 * i + 1] = make_float2(f.z, f.w);
-    }
-  }
-  float wq[8], wk[8];
-  if (here) {
-    load_weight8<T>(p.weight[0], p.weight_f32, c, wq);
-    load_weight8<T>(p.weight[1], p.weight_f32, c, wk);
-  }
+  for (int h = 0; h < CH; ++h) here[h] = c + h * apart < p.D;
 
+  uint4 raw[kSteps][CH];
 #pragma unroll
-  for (int r = 0; r < kRopeRows; ++r) {
-    const uint32_t v[4] = {raw[r].x, raw[r].y, raw[r].z, raw[r].w};
-    float x[8];
+  for (int r = 0; r < kSteps; ++r)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Pack16<T>::unpack(v[i]);
-      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    for (int h = 0; h < CH; ++h) {
+      raw[r][h] = make_uint4(0, 0, 0, 0);
+      if (here[h] && row0 + r * per < heads)
+        raw[r][h] = *reinterpret_cast<const uint4*>(in + r * per * in_h + h * apart);
     }
-    if (p.norm) {
-      float sum = 0.0f;
+
+  // out[i] = mine[i] x[i] + other[i] x[i's partner]
+  float mine[8 * CH], other[8 * CH];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-      for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float inv = rsqrtf(sum / static_cast<float>(p.D) + p.eps);
+  for (int h = 0; h < CH; ++h) {
+    float w[8] = {};
+    if (here[h]) load_weight8<T>(is_k ? p.weight[1] : p.weight[0], p.weight_f32, c + h * apart, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * (which[r] == 1 ? wk[i] : wq[i]);
-    }
-    if (p.table) {  // uniform
-      if (INTERLEAVED) {
-        if (turns) {
+    for (int i = 0; i < 8; ++i) mine[8 * h + i] = w[i];
+  }
+  if (p.table && turns) {
+    const float4* src =
+        reinterpret_cast<const float4*>(p.table + t * p.ld_table + (INTERLEAVED ? c >> 1 : c));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = a * cs[i % kPairs].x - b * cs[i % kPairs].y;
-            x[2 * i + 1] = b * cs[i % kPairs].x + a * cs[i % kPairs].y;
-          }
-        }
-      } else {
-        const int partner = (lane & ~(lanes - 1)) | (turns ? (second ? at - (half >> 3) : at + (half >> 3)) : at);
+    for (int i = 0; i < 2 * CH; ++i) {
+      const float4 f = __ldg(src + i);
+      const float cs[2] = {f.x, f.z}, sn[2] = {f.y, f.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float o = __shfl_sync(0xffffffffu, x[i], partner);
-          if (turns) x[i] = x[i] * cs[i % kPairs].x + (second ? o : -o) * cs[i % kPairs].y;
-        }
+      for (int k = 0; k < 2; ++k) {
+        const int a = INTERLEAVED ? 4 * i + 2 * k : 2 * i + k, b = a + kPartner;
+        const float wa = mine[a], wb = mine[b];
+        mine[a] = wa * cs[k], other[a] = -wb * sn[k];
+        mine[b] = wb * cs[k], other[b] = wa * sn[k];
       }
     }
-    if (here && which[r] >= 0) {
-      const int w = which[r];
-      uint4 u;
-      u.x = Pack16<T>::pack(x[0], x[1]);
-      u.y = Pack16<T>::pack(x[2], x[3]);
-      u.z = Pack16<T>::pack(x[4], x[5]);
-      u.w = Pack16<T>::pack(x[6], x[7]);
-      *reinterpret_cast<uint4*>(static_cast<T*>(w ? p.out[1] : p.out[0]) + t * (w ? p.out_t[1] : p.out_t[0]) +
-                                head[r] * (w ? p.out_h[1] : p.out_h[0]) + c) = u;
+  }
+
+#pragma unroll
+  for (int r = 0; r < kSteps; ++r) {
+    float x[8 * CH], y[8 * CH];
+#pragma unroll
+    for (int h = 0; h < CH; ++h) {
+      const uint32_t v[4] = {raw[r][h].x, raw[r][h].y, raw[r][h].z, raw[r][h].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = Pack16<T>::unpack(v[i]);
+        x[8 * h + 2 * i] = f.x, x[8 * h + 2 * i + 1] = f.y;
+      }
     }
+    if (p.norm) {
+      float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8 * CH; i += 2) s0 = fmaf(x[i], x[i], s0), s1 = fmaf(x[i + 1], x[i + 1], s1);
+      float sum = s0 + s1;
+      for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float inv = rsqrtf(fmaf(sum, p.inv_D, p.eps));
+#pragma unroll
+      for (int i = 0; i < 8 * CH; ++i) x[i] *= inv;
+    }
+    if (p.table && turns) {
+#pragma unroll
+      for (int i = 0; i < 8 * CH; ++i) y[i] = fmaf(x[i], mine[i], x[i ^ kPartner] * other[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8 * CH; ++i) y[i] = x[i] * mine[i];
+    }
+#pragma unroll
+    for (int h = 0; h < CH; ++h)
+      if (here[h] && row0 + r * per < heads) {
+        uint4 u;
+        u.x = Pack16<T>::pack(y[8 * h], y[8 * h + 1]);
+        u.y = Pack16<T>::pack(y[8 * h + 2], y[8 * h + 3]);
+        u.z = Pack16<T>::pack(y[8 * h + 4], y[8 * h + 5]);
+        u.w = Pack16<T>::pack(y[8 * h + 6], y[8 * h + 7]);
+        *reinterpret_cast<uint4*>(out + r * per * out_h + h * apart) = u;
+      }
   }
 }
 
