@@ -46,10 +46,11 @@ constexpr int kMaxShares = 192;  // most CTAs that share the last items evenly
 template <int NP>
 struct AttnCfg {  // NP: 64-channel panels of a head (1: D <= 64, 2: D <= 128)
   static constexpr int kTileBytes = NP * kAtPanelBytes;
-  static constexpr int kStages = NP == 2 ? 5 : 8;
-  static constexpr int kNumBars = 2 * kStages + 20 + 2 * kItems;
-  static constexpr int kSmallBytes = 8 * kNumBars + kItems * 48 + 2 * 16 + 4 * (kMaxShares + 1) + 16;
-  static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + kSmallBytes + 1024;
+  static constexpr int kStages = NP == 2 ? 4 : 8;
+  static constexpr int kStageOut = 4096;  // output staging of a warp: 32 rows of 128 bytes
+  static constexpr int kNumBars = 2 * kStages + 19 + 3 * kItems;
+  static constexpr int kSmallBytes = 8 * kNumBars + kItems * 48 + 2 * 16 + 5 * kMaxShares + 4 + 16;
+  static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 8 * kStageOut + kSmallBytes + 1024;
   static constexpr int kO = 256;  // TMEM columns from S_i to O_i
 };
 
@@ -152,8 +153,16 @@ struct AttnWalk {
   int block = 0;
 
   __device__ __forceinline__ bool find(const AttnParams& p, int item, int lane, AttnPlace& a) {
-    if (item < base) base = block = 0;
     const int span = 2 * p.positions;
+    if (!p.cu_q) {
+      a.q0 = a.k0 = 0;
+      a.lq = p.Tq;
+      a.lk = p.Tk;
+      if (item >= (p.Tq + span - 1) / span * p.heads_kv) return false;
+      attn_place(p, item, a);
+      return true;
+    }
+    if (item < base) base = block = 0;
     while (block < p.batch) {
       const int b = block + lane;
       int q0 = 0, lq = 0, k0 = 0, lk = 0;
@@ -199,24 +208,69 @@ __device__ __forceinline__ int attn_count(const AttnParams& p, int lane) {
   return __reduce_add_sync(0xffffffffu, n) * p.heads_kv;
 }
 
-// Even division of the last items.  pre[x] is the work before item x of them (`items` of them, `total` in all); share s
-// of `shares` begins at edge(s): at a whole step of the item that it falls into, or at that item's edge if little would
-// be cut off.
+// Even division of the last items.  pre[x] is the work before item x of them (`items` of them, `total` in all) and
+// units[x] the work of one of its steps; share s of `shares` begins at edge(s): at a whole step of the item that it falls
+// into, or at that item's edge if little would be cut off.
 struct AttnShares {
-  const int* pre;
+  int* pre;
+  uint8_t* units;
   int items, total, shares;
 
+  // Fills pre and units for the items from number `first` on (the whole warp).
+  __device__ __forceinline__ void divide(const AttnParams& p, const AttnWalk& walk, int first, int lane) {
+    const int span = 2 * p.positions;
+    total = 0;
+    if (lane == 0) pre[0] = 0;
+#pragma unroll 1
+    for (int k = 0; k < items; k += 32) {
+      int base = walk.base, work = 0, unit = 1;
+#pragma unroll 1
+      for (int b = walk.block; b < p.batch && base < first + items; ++b) {
+        AttnPlace a;
+        attn_bounds(p.cu_q, b, p.Tq, a.q0, a.lq);
+        attn_bounds(p.cu_k, b, p.Tk, a.k0, a.lk);
+        const int n = (a.lq + span - 1) / span * p.heads_kv, x = first + k + lane - base;
+        if (x >= 0 && x < n) {
+          attn_place(p, x, a);
+          work = attn_work(p, a);
+          unit = attn_unit(p, a);
+        }
+        base += n;
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, work, o);
+        if (lane >= o) work += v;
+      }
+      if (k + lane < items) {
+        pre[k + lane + 1] = total + work;
+        units[k + lane] = static_cast<uint8_t>(unit);
+      }
+      total += __shfl_sync(0xffffffffu, work, min(31, items - k - 1));
+    }
+    __syncwarp();
+    // A share of less than 8 units costs more than it saves, unless it is an item of its own.  (No two edges can fall on
+    // one step: they are at least two units apart.)
+    shares = max(1, min(p.shares, max(total / 8, min(items, total / 2))));
+  }
   __device__ __forceinline__ int item_at(int x, int lane) const {  // the item that work unit x < total lies in
     int n = 0;
+#pragma unroll 1
     for (int i = 0; i < items; i += 32)
       n += __popc(__ballot_sync(0xffffffffu, i + lane < items && pre[i + lane + 1] <= x));
     return n;
   }
-  __device__ __forceinline__ int edge(int s, int unit_of_item, int i) const {
-    const int x = static_cast<int>(static_cast<int64_t>(total) * s / shares);
-    const int a = pre[i], e = pre[i + 1];
-    if (x - a < 4 || e - x < 4) return x - a < e - x ? a : e;
-    return a + (x - a + unit_of_item - 1) / unit_of_item * unit_of_item;
+  __device__ __forceinline__ int snap(int x, int from, int upto, int unit) const {
+    if (x - from < 4 || upto - x < 4) return x - from < upto - x ? from : upto;
+    return from + (x - from + unit - 1) / unit * unit;
+  }
+  __device__ __forceinline__ int place(int s) const {  // before it is moved to a step
+    return static_cast<int>(static_cast<int64_t>(total) * s / shares);
+  }
+  __device__ __forceinline__ int edge(int s, int lane) const {
+    if (s >= shares) return total;
+    const int x = place(s), i = item_at(x, lane);
+    return snap(x, pre[i], pre[i + 1], units[i]);
   }
 };
 
@@ -463,12 +517,14 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(attn_smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_smem = smem;                      // two query tiles
   uint8_t* ring = smem + 2 * Cfg::kTileBytes;  // key and value tiles in turn
-  uint8_t* small = ring + S * Cfg::kTileBytes;
+  uint8_t* staging = ring + S * Cfg::kTileBytes;
+  uint8_t* small = staging + 8 * Cfg::kStageOut;
   AttnItem* item_smem = reinterpret_cast<AttnItem*>(small);              // [kItems]
   const uint32_t answers = smem_u32(small + kItems * sizeof(AttnItem));       // [2] of launch control
   uint64_t* bars = reinterpret_cast<uint64_t*>(small + kItems * sizeof(AttnItem) + 32);
   int* pre = reinterpret_cast<int*>(bars + Cfg::kNumBars);
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pre + kMaxShares + 1);
+  uint8_t* units = reinterpret_cast<uint8_t*>(pre + kMaxShares + 1);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(units + kMaxShares);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   const uint32_t bar0 = smem_u32(bars);
   auto kv_full = [&](int s) { return bar0 + 8 * s; };
@@ -483,10 +539,10 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   const uint32_t drain = bar0 + 8 * (2 * S + 14);
   const uint32_t twin_ready = bar0 + 8 * (2 * S + 15);  // tile 1's part of a twin item is in TMEM
   const uint32_t twin_done = bar0 + 8 * (2 * S + 16);   // and was read
-  const uint32_t want = bar0 + 8 * (2 * S + 17);        // the producer has issued all loads of its item
-  auto answer_full = [&](int i) { return bar0 + 8 * (2 * S + 18 + i); };
-  auto item_full = [&](int i) { return bar0 + 8 * (2 * S + 20 + i); };
-  auto item_empty = [&](int i) { return bar0 + 8 * (2 * S + 20 + kItems + i); };
+  auto answer_full = [&](int i) { return bar0 + 8 * (2 * S + 17 + i); };
+  auto item_full = [&](int i) { return bar0 + 8 * (2 * S + 19 + i); };
+  auto item_empty = [&](int i) { return bar0 + 8 * (2 * S + 19 + kItems + i); };
+  auto want = [&](int i) { return bar0 + 8 * (2 * S + 19 + 2 * kItems + i); };  // the item's loads are all issued
   constexpr int kReaders = 11;                          // warps that read an item: all but the scheduler
 
   const int warp = uniform(threadIdx.x >> 5);
@@ -495,7 +551,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   if (threadIdx.x == 0) {
     for (int b = 0; b < Cfg::kNumBars; ++b) {
       const int c = b - 2 * S;
-      mbar_init(&bars[b], (c >= 8 && c < 12) || c == 15 || c == 16 ? 4 : c >= 20 + kItems ? kReaders : 1);
+      mbar_init(&bars[b], (c >= 8 && c < 12) || c == 15 || c == 16 ? 4 : c >= 19 + kItems && c < 19 + 2 * kItems ? kReaders : 1);
     }
     *abort_flag = 0;
     fence_mbarrier_init();
@@ -542,16 +598,19 @@ __global__ void __launch_bounds__(kAtThreads, 1)
     setmaxnreg_dec<56>();
     if (warp == 11) {
       // -------------------------------------------------------------- scheduler
+      // (One call site for each piece of work: the instruction cache is shared with the loops that matter.  Unrolled and
+      // called from several places this warp's code was 66 of the kernel's 157 KB, and every cold path ran at 10 to 15
+      // cycles an instruction.)
       AttnWalk walk;
       AttnPlace a;
       const int items = attn_count(p, lane);
       const int whole = p.shares > 0 ? items / p.shares * p.shares : items;
-      AttnShares sh{pre, items - whole, 0, 0};
+      AttnShares sh{pre, units, items - whole, 0, 0};
       uint32_t sent = 0, asked = 0;
+      bool brief = false;
       auto send = [&](const AttnItem& x) {
         const int at = sent % kItems;
         guard.wait(item_empty(at), ((sent / kItems) & 1) ^ 1);
-        if (sent > 0) guard.wait(want, (sent - 1) & 1);
         if (lane == 0) {
           int4* dst = reinterpret_cast<int4*>(item_smem + at);
           dst[0] = make_int4(x.q_row, x.left, x.k_row, x.keys);
@@ -562,110 +621,72 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         __syncwarp();
         ++sent;
       };
-      // steps [lo, hi) of the item at place a, as part `part` or as a whole (-1)
-      auto send_steps = [&](int lo, int hi, int part) {
-        AttnItem x;
-        const int n0 = attn_tiles(p, a, a.pos), n1 = attn_tiles(p, a, a.pos + p.positions);
-        const int first = lo * kAtTile;
-        x.q_row = a.q0 + a.pos;
-        x.left = a.lq - a.pos;
-        x.k_row = a.k0 + first;
-        x.keys = a.lk - first;
-        x.head = a.head;
-        x.see = (p.causal ? a.pos + a.lk - a.lq + 1 : a.lk) - first;
-        x.nt[0] = max(min(n0, hi) - lo, 0);
-        x.nt[1] = max(min(n1, hi) - lo, 0);
-        x.twin = x.left <= p.positions && x.nt[0] > 1;
-        const int n = max(x.nt[0], x.nt[1]);
-        x.fixing = n > 0 && n * kAtTile > x.keys && a.k0 + a.lk < p.Tk;
-        if (x.twin) {
-          x.nt[1] = n / 2;
-          x.nt[0] = n - x.nt[1];
-        }
-        x.part = part;
-        x.valid = 1;
-        send(x);
-      };
-      // Works out the division of the last items: their work, lane by lane, and its prefix.
-      auto divide = [&]() {
-        if (!walk.find(p, whole, lane, a)) return;  // (none are left)
-        int work[kMaxShares / 32];
-#pragma unroll
-        for (int k = 0; k < kMaxShares / 32; ++k) work[k] = 0;
-        int base = 0, b = walk.block;
-        base = walk.base;
-        const int span = 2 * p.positions;
-        for (; b < p.batch && base < items; ++b) {
-          AttnPlace at;
-          attn_bounds(p.cu_q, b, p.Tq, at.q0, at.lq);
-          attn_bounds(p.cu_k, b, p.Tk, at.k0, at.lk);
-          const int n = (at.lq + span - 1) / span * p.heads_kv;
-#pragma unroll
-          for (int k = 0; k < kMaxShares / 32; ++k) {
-            const int x = whole + 32 * k + lane - base;
-            if (x >= 0 && x < n) {
-              attn_place(p, x, at);
-              work[k] = attn_work(p, at);
-            }
-          }
-          base += n;
-        }
-        int total = 0;
-        if (lane == 0) pre[0] = 0;
-#pragma unroll
-        for (int k = 0; k < kMaxShares / 32; ++k) {
-          int upto = work[k];
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-          }
-          if (32 * k + lane < sh.items) pre[32 * k + lane + 1] = total + upto;
-          total += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        __syncwarp();
-        sh.total = total;
-        // A share of less than 8 units costs more than it saves, unless it is an item of its own.  (No two edges can fall
-        // on one step: they are at least two units apart.)
-        sh.shares = max(1, min(p.shares, max(total / 8, min(sh.items, total / 2))));
-      };
       int v = blockIdx.x;
+#pragma unroll 1
       while (v >= 0) {
-        if (v < whole) {
-          walk.find(p, v, lane, a);
-          send_steps(0, 0x7fffff, -1);
-        } else if (p.shares > 0 && v < whole + p.shares) {
-          const int s = v - whole;
-          if (sh.shares == 0) divide();
-          if (s == 0) {  // for the kernel that joins the parts
-            for (int x = lane; x <= sh.items; x += 32) p.meta[4 + x] = sh.items ? pre[x] : 0;
-            if (lane == 0) p.meta[0] = sh.shares, p.meta[1] = sh.items, p.meta[2] = whole;
-          }
-          if (s < sh.shares) {
-            auto edge = [&](int t) {
-              const int64_t x = static_cast<int64_t>(sh.total) * t / sh.shares;
-              if (t >= sh.shares) return sh.total;
-              const int i = sh.item_at(static_cast<int>(x), lane);
-              walk.find(p, whole + i, lane, a);
-              return sh.edge(t, attn_unit(p, a), i);
-            };
-            const int begin = edge(s), end = edge(s + 1);
-            for (int x = begin; x < end;) {
-              const int i = sh.item_at(x, lane);
-              walk.find(p, whole + i, lane, a);
-              const int unit = attn_unit(p, a), from = pre[i], upto = min(pre[i + 1], end);
-              const bool part = x > from || upto < pre[i + 1];
-              send_steps((x - from) / unit, (upto - from) / unit, part ? 2 * s + (x > from ? 0 : 1) : -1);
-              x = upto;
+        const int s = v - whole;
+        int x = 0, end = 1;  // a whole item, or the share [x, end) of the last ones
+        if (s >= 0) {
+          end = 0;
+          if (s < p.shares) {
+            if (sh.shares == 0) sh.divide(p, walk, whole, lane);
+            if (s == 0) {  // for the kernel that joins the parts
+              for (int i = lane; i <= sh.items; i += 32) p.meta[4 + i] = sh.items ? pre[i] : 0;
+              if (lane == 0) p.meta[0] = sh.shares, p.meta[1] = sh.items, p.meta[2] = whole;
+            }
+            if (s < sh.shares) {
+#pragma unroll 1
+              for (int k = 0; k < 2; ++k) {
+                x = end;
+                end = sh.edge(s + k, lane);
+              }
             }
           }
         }
-        // The next one, once this one's loads are all under way (a few steps before its end): asked for earlier, it
-        // would be taken from CTAs that are free sooner.
-        if (sent > 0) guard.wait(want, (sent - 1) & 1);
+#pragma unroll 1
+        while (x < end) {
+          int index = v, lo = 0, hi = 0x7fffffff, part = -1, next = end;
+          if (s >= 0) {
+            const int i = sh.item_at(x, lane), from = pre[i], upto = pre[i + 1], shift = units[i] - 1;
+            next = min(upto, end);
+            index = whole + i;
+            lo = (x - from) >> shift;
+            hi = (next - from) >> shift;
+            if (x > from || next < upto) part = 2 * s + (x > from ? 0 : 1);
+          }
+          x = next;
+          if (!walk.find(p, index, lane, a)) continue;
+          AttnItem it;
+          const int n0 = attn_tiles(p, a, a.pos), n1 = attn_tiles(p, a, a.pos + p.positions);
+          const int first = lo * kAtTile;
+          it.q_row = a.q0 + a.pos;
+          it.left = a.lq - a.pos;
+          it.k_row = a.k0 + first;
+          it.keys = a.lk - first;
+          it.head = a.head;
+          it.see = (p.causal ? a.pos + a.lk - a.lq + 1 : a.lk) - first;
+          it.nt[0] = max(min(n0, hi) - lo, 0);
+          it.nt[1] = max(min(n1, hi) - lo, 0);
+          it.twin = it.left <= p.positions && it.nt[0] > 1;
+          const int n = max(it.nt[0], it.nt[1]);
+          it.fixing = n > 0 && n * kAtTile > it.keys && a.k0 + a.lk < p.Tk;
+          if (it.twin) {
+            it.nt[1] = n / 2;
+            it.nt[0] = n - it.nt[1];
+          }
+          it.part = part;
+          it.valid = 1;
+          brief = n <= 8;
+          send(it);
+        }
+        // The next one, once this one's loads are all under way (two steps before its end): asked for earlier, it would
+        // be taken from CTAs that are free sooner.  Short items are asked for one ahead, since finding one takes as long
+        // as three steps.
+        const uint32_t behind = brief ? 2 : 1;
+        if (sent >= behind) guard.wait(want((sent - behind) % kItems), ((sent - behind) / kItems) & 1);
         const int slot = asked & 1;
         if (lane == 0) {
-          mbar_arrive_expect_tx(bars + 2 * S + 18 + slot, 16);
+          mbar_arrive_expect_tx(bars + 2 * S + 17 + slot, 16);
           launch_cancel(answers + 16 * slot, answer_full(slot));
         }
         __syncwarp();
@@ -676,10 +697,8 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         ++asked;
         if (guard.aborted()) v = -1;
       }
-      AttnItem end;
-      end.q_row = end.left = end.k_row = end.keys = end.head = end.see = end.nt[0] = end.nt[1] = 0;
-      end.twin = end.fixing = end.part = end.valid = 0;
-      send(end);
+      AttnItem over = {};
+      send(over);
     } else if (warp == 9) {
       // -------------------------------------------------------------- TMA producer
       uint32_t stage = 0, phase = 0, issued_mask = 0, issued_parity = 0;
@@ -698,40 +717,33 @@ __global__ void __launch_bounds__(kAtThreads, 1)
                           it.q_row + i * p.positions);
             ++q_count[i];
           };
-          auto load_kv = [&](const CUtensorMap* map, int tile) {
-            if (stop) return;
+          const bool twin = it.twin != 0;
+          const int n = twin ? it.nt[0] + it.nt[1] : max(it.nt[0], it.nt[1]);
+          // K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 K3 ... V(n-2) V(n-1) for a twin; Q0 before K0, Q1 behind it
+#pragma unroll 1
+          for (int x = 0; !stop && x < 2 * n; ++x) {
+            if (x < 2) {
+              if ((x == 0 ? it.nt[0] : it.nt[1]) > 0 && !(twin && x == 1)) load_q(x);
+              if (stop) break;
+            }
+            const int y = x - 2;
+            const bool value = twin ? y >= 0 && ((y & 1) == 0 || (y >> 1) + 2 >= n) : (x & 1) != 0;
+            const int tile = !twin ? x >> 1 : y < 0 ? x : (y & 1) == 0 ? y >> 1 : min((y >> 1) + 2, n - 1);
             guard.wait(kv_empty(stage), phase ^ 1);
-            if ((stop = guard.aborted())) return;
+            if ((stop = guard.aborted())) break;
             uint64_t* full = bars + stage;
             mbar_arrive_expect_tx(full, Cfg::kTileBytes);
             for (int c = 0; c < NP; ++c)
-              tma_load_3d(ring + stage * Cfg::kTileBytes + c * kAtPanelBytes, map, full, c * 64, it.head,
-                          it.k_row + tile * kAtTile);
+              tma_load_3d(ring + stage * Cfg::kTileBytes + c * kAtPanelBytes, value ? &tmap_v : &tmap_k, full, c * 64,
+                          it.head, it.k_row + tile * kAtTile);
             issued_mask |= 1u << stage;
             issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
             if (++stage == S) {
               stage = 0;
               phase ^= 1;
             }
-          };
-          if (it.nt[0] > 0) load_q(0);
-          if (it.twin) {  // K0 K1 | V0 K2 V1 K3 | V2 ...
-            const int n = it.nt[0] + it.nt[1];
-            load_kv(&tmap_k, 0);
-            load_kv(&tmap_k, 1);
-            for (int t = 0; !stop && t < n; ++t) {
-              load_kv(&tmap_v, t);
-              if (t + 2 < n) load_kv(&tmap_k, t + 2);
-            }
-          } else {  // K0 V0 | K1 V1 | ...
-            const int n = max(it.nt[0], it.nt[1]);
-            for (int j = 0; !stop && j < n; ++j) {
-              load_kv(&tmap_k, j);
-              if (!stop && j == 0 && it.nt[1] > 0) load_q(1);
-              load_kv(&tmap_v, j);
-            }
           }
-          bar_arrive(want);
+          bar_arrive(want((item_count - 1) % kItems));
         }
         __syncwarp();
       }
@@ -755,7 +767,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       const uint64_t v_desc = make_nmajor_desc(smem_u32(ring), kAtPanelBytes);
       constexpr uint32_t kTileStep = Cfg::kTileBytes >> 4;
       uint32_t slot = 0, slot_phase = 0;  // next ring slot to be consumed
-      uint32_t q_count[2] = {0, 0}, p_count[2] = {0, 0}, fixes = 0;
+      uint32_t q_phase = 0, p_phase = 0, fixes = 0;  // a bit for each tile
       auto take = [&](uint32_t& s, uint32_t& phase) {  // the next ring slot, in load order
         s = slot;
         phase = slot_phase;
@@ -779,80 +791,80 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         const int n = max(it.nt[0], it.nt[1]), all = it.nt[0] + it.nt[1];
         if (n == 0) continue;
         uint32_t ks = 0, kph = 0, vs = 0, vph = 0;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
+          const int mine = i == 0 ? it.nt[0] : it.nt[1], q = twin ? 0 : i;
           if (i == 0 || twin) {
             take(ks, kph);
             guard.wait(kv_full(ks), kph);
           }
-          if (it.nt[i] > 0 && !(i == 1 && twin)) {
-            guard.wait(q_full(i), q_count[i] & 1);
-            ++q_count[i];
+          if (mine > 0 && q == i) {
+            guard.wait(q_full(i), q_phase >> i & 1);
+            q_phase ^= 1u << i;
           }
           tc_fence_after();
           if (elect_one()) {
-            if (it.nt[i] > 0) qk(i, twin ? 0 : i, ks);
-            if (twin ? all == 2 && i == 1 : it.nt[i] == 1) bar_commit(q_empty(twin ? 0 : i));
+            if (mine > 0) qk(i, q, ks);
+            if (twin ? all == 2 && i == 1 : mine == 1) bar_commit(q_empty(q));
             if (i == 1 || twin) bar_commit(kv_empty(ks));
           }
           __syncwarp();
         }
-        for (int j = 0; j < n; ++j) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const bool works = j < it.nt[i], ends = j + 1 >= it.nt[i];
-            if (twin && !works) continue;
-            const int tile = twin ? 2 * j + i : j;  // key tile whose weights are multiplied
-            const bool has_k = twin ? tile + 2 < all : j + 1 < n;
-            if (i == 0 || twin) {
-              take(vs, vph);
-              if (has_k) {  // (the loads run ahead: neither wait lasts)
-                take(ks, kph);
-                guard.both(kv_full(vs), vph, kv_full(ks), kph);
-              } else {
-                guard.wait(kv_full(vs), vph);
-              }
-              // cleared by warp 10 while the softmax still works on this tile
-              if (it.fixing && tile + 1 == (twin ? all : n)) {
-                if (lane == 0) bar_arrive(v_need);
-                guard.wait(v_fixed, fixes & 1);
-                ++fixes;
-              }
+#pragma unroll 1
+        for (int step = 0; step < 2 * n; ++step) {
+          const int i = step & 1, j = step >> 1, mine = i == 0 ? it.nt[0] : it.nt[1], q = twin ? 0 : i;
+          const bool works = j < mine, ends = j + 1 >= mine;
+          if (twin && !works) continue;
+          const int tile = twin ? step : j;  // key tile whose weights are multiplied
+          const bool has_k = twin ? tile + 2 < all : j + 1 < n;
+          if (i == 0 || twin) {
+            take(vs, vph);
+            if (has_k) {  // (the loads run ahead: neither wait lasts)
+              take(ks, kph);
+              guard.both(kv_full(vs), vph, kv_full(ks), kph);
+            } else {
+              guard.wait(kv_full(vs), vph);
             }
-            const uint64_t b0 = v_desc + vs * kTileStep;
-            const uint32_t d = tmem + Cfg::kO + i * 128, a0 = tmem + i * 128;
-            if (works) {
-              guard.wait(p_full(i, 0), p_count[i] & 1);
-              tc_fence_after();
-              if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < kFirstSteps; ++k)
-                  mma_f16_ts(d, a0 + k * 8, b0 + ((k * 16 * 128) >> 4), idesc_pv, k > 0 ? 1 : j > 0);
-              }
-              __syncwarp();
-              guard.wait(p_full(i, 1), p_count[i] & 1);
-              ++p_count[i];
-              tc_fence_after();
+            // cleared by warp 10 while the softmax still works on this tile
+            if (it.fixing && tile + 1 == (twin ? all : n)) {
+              if (lane == 0) bar_arrive(v_need);
+              guard.wait(v_fixed, fixes & 1);
+              ++fixes;
             }
+          }
+          const uint64_t b0 = v_desc + vs * kTileStep;
+          const uint32_t d = tmem + Cfg::kO + i * 128, a0 = tmem + i * 128;
+          if (works) {
+            guard.wait(p_full(i, 0), p_phase >> i & 1);
+            tc_fence_after();
             if (elect_one()) {
-              if (works) {
 #pragma unroll
-                for (int k = kFirstSteps; k < 8; ++k)
-                  mma_f16_ts(d, a0 + k * 8, b0 + ((k * 16 * 128) >> 4), idesc_pv, 1);
-                if (ends) {
-                  bar_commit(o_full(i));
-                } else {
-                  qk(i, twin ? 0 : i, ks);
-                  if (twin ? tile + 3 == all : j + 2 == it.nt[i]) bar_commit(q_empty(twin ? 0 : i));
-                }
-              }
-              if (i == 1 || twin) {  // all that read the slots are issued
-                bar_commit(kv_empty(vs));
-                if (has_k) bar_commit(kv_empty(ks));
-              }
+              for (int k = 0; k < kFirstSteps; ++k)
+                mma_f16_ts(d, a0 + k * 8, b0 + ((k * 16 * 128) >> 4), idesc_pv, k > 0 ? 1 : j > 0);
             }
             __syncwarp();
+            guard.wait(p_full(i, 1), p_phase >> i & 1);
+            p_phase ^= 1u << i;
+            tc_fence_after();
           }
+          if (elect_one()) {
+            if (works) {
+#pragma unroll
+              for (int k = kFirstSteps; k < 8; ++k)
+                mma_f16_ts(d, a0 + k * 8, b0 + ((k * 16 * 128) >> 4), idesc_pv, 1);
+              if (ends) {
+                bar_commit(o_full(i));
+              } else {
+                qk(i, q, ks);
+                if (twin ? tile + 3 == all : j + 2 == mine) bar_commit(q_empty(q));
+              }
+            }
+            if (i == 1 || twin) {  // all that read the slots are issued
+              bar_commit(kv_empty(vs));
+              if (has_k) bar_commit(kv_empty(ks));
+            }
+          }
+          __syncwarp();
         }
       }
       if (guard.aborted()) {  // the products still in flight read shared memory and TMEM
@@ -928,18 +940,28 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         }
         tc_fence_after();
         const int tile = twin ? 2 * j + i : j;
+        if (tile >= full) {
+          // Scores that a row does not see become -infinity in place, 32 columns at a time (a loop, not 128 selects in a
+          // row: seldom run, straight code costs ten cycles and more an instruction to fetch).
+          const int seen = keys - tile * kAtTile;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const int left = seen - c * 32;
+            if (!__any_sync(0xffffffffu, left < 32)) continue;
+            const uint32_t sees = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+            uint32_t x[32];
+            tmem_ld_32x32b_x32(s_addr + c * 32, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = sees >> e & 1u ? x[e] : 0xff800000u;
+            tmem_st_32x32b_x32(s_addr + c * 32, x);
+          }
+          tmem_st_wait();
+        }
         uint32_t s[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
         tmem_ld_wait();
-        if (tile >= full) {
-          const int seen = keys - tile * kAtTile;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c * 32 + e >= seen) s[c][e] = 0xff800000u;
-        }
         // The first half of the weights is taken with the maximum so far, while the tile's own maximum is still being
         // found: it seldom grows enough to matter, and then the half is taken again.  Finding the maximum first would
         // leave the special-function unit idle meanwhile.
@@ -1038,6 +1060,49 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         const int64_t t = item->q_row + (twin ? 0 : i * p.positions) + in_tile;
         const int head = item->head * p.group + r - in_tile * p.group;
         const int64_t part = static_cast<int64_t>(item->part) * 256 + i * 128 + row;
+        if (valid) {
+          const float lse2 = l == 0.0f ? -CUDART_INF_F : fmaf(m, c2, log2f(l));
+          if (parts)
+            p.part_lse[part] = lse2;
+          else if (p.lse)
+            p.lse[t * (p.heads_kv * p.group) + head] = lse2 * 0.69314718055994530942f;
+        }
+        // Rows go out through the warp's staging buffer, 128 bytes of 32 rows at a time, so that eight lanes write 128
+        // bytes of a row together (16 bytes of each lane's own row per store took 8000 cycles for a tile, and held up
+        // every other access of the SM meanwhile).
+        uint64_t base = parts ? reinterpret_cast<uint64_t>(p.part_o + part * p.D)
+                              : reinterpret_cast<uint64_t>(static_cast<T*>(p.out) + t * p.out_t + head * p.out_h);
+        if (!valid) base = 0;
+        const int row_bytes = p.D * (parts ? 4 : 2);
+        const uint32_t stage = smem_u32(staging + warp * Cfg::kStageOut);
+        auto put = [&](int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {  // 16 bytes of this lane's row
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 +
+                                                                        ((piece ^ (lane & 7)) << 4)),
+                       "r"(a), "r"(b), "r"(c), "r"(d)
+                       : "memory");
+        };
+        auto write_out = [&](int from) {  // bytes [from, from + 128) of the rows
+          __syncwarp();
+          const int at = from + (lane & 7) * 16;
+          uint32_t v[8][4];
+          uint64_t to[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int src = 4 * k + (lane >> 3);
+            to[k] = __shfl_sync(0xffffffffu, base, src);
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v[k][0]), "=r"(v[k][1]), "=r"(v[k][2]), "=r"(v[k][3])
+                         : "r"(stage + src * 128 + (((lane & 7) ^ (src & 7)) << 4))
+                         : "memory");
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (to[k] && at < row_bytes)
+              asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(to[k] + at), "r"(v[k][0]), "r"(v[k][1]),
+                           "r"(v[k][2]), "r"(v[k][3])
+                           : "memory");
+          __syncwarp();
+        };
 #pragma unroll 1
         for (int c = 0; c < 2 * NP; ++c) {
           uint32_t o[32];
@@ -1056,34 +1121,21 @@ __global__ void __launch_bounds__(kAtThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0);
           }
-          if (!valid) continue;
+          if (!__all_sync(0xffffffffu, any)) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            const int col = c * 32 + e;
-            if (col >= p.D) continue;
-            float f[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = any ? __uint_as_float(o[e + k]) : 0.0f;
-            if (parts) {
-              float4* dst = reinterpret_cast<float4*>(p.part_o + part * p.D + col);
-              dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-              dst[1] = make_float4(f[4], f[5], f[6], f[7]);
-            } else {
-              uint4 u;
-              u.x = Pack16<T>::pack(f[0], f[1]);
-              u.y = Pack16<T>::pack(f[2], f[3]);
-              u.z = Pack16<T>::pack(f[4], f[5]);
-              u.w = Pack16<T>::pack(f[6], f[7]);
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + t * p.out_t + head * p.out_h + col) = u;
-            }
+            for (int e = 0; e < 32; ++e) o[e] = any ? o[e] : 0;
           }
-        }
-        if (valid) {
-          const float lse2 = l == 0.0f ? -CUDART_INF_F : fmaf(m, c2, log2f(l));
-          if (parts)
-            p.part_lse[part] = lse2;
-          else if (p.lse)
-            p.lse[t * (p.heads_kv * p.group) + head] = lse2 * 0.69314718055994530942f;
+          if (parts) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) put(e, o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else {
+            auto two = [&](int e) { return Pack16<T>::pack(__uint_as_float(o[e]), __uint_as_float(o[e + 1])); };
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              put((c & 1) * 4 + e, two(8 * e), two(8 * e + 2), two(8 * e + 4), two(8 * e + 6));
+            if (!(c & 1)) continue;
+          }
+          write_out((parts ? c : c >> 1) * 128);
         }
       }
       if (twin) {
@@ -1112,8 +1164,8 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_con
   const int shares = p.meta[0], items = p.meta[1], whole = p.meta[2], x = blockIdx.x;
   // (the limits also hold if the first kernel gave up and left no plan)
   if (x >= items || items >= kMaxShares || shares < 1 || shares > p.shares) return;
-  const int* pre = p.meta + 4;
-  const AttnShares sh{pre, items, pre[items], shares};
+  int* pre = p.meta + 4;
+  const AttnShares sh{pre, nullptr, items, pre[items], shares};
   const int from = pre[x], upto = pre[x + 1];
   AttnWalk walk;
   AttnPlace a;
@@ -1122,8 +1174,8 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_con
   // the edges that lie inside this item
   int s = max(1, static_cast<int>((static_cast<int64_t>(from) * shares + sh.total - 1) / max(sh.total, 1)));
   int first = 0, last = -1;  // shares of the item, if it was divided
-  for (; s < shares && static_cast<int64_t>(sh.total) * s / shares < upto; ++s) {
-    const int e = sh.edge(s, unit, x);
+  for (; s < shares && sh.place(s) < upto; ++s) {
+    const int e = sh.snap(sh.place(s), from, upto, unit);
     if (e <= from || e >= upto) continue;
     if (last < 0) first = s - 1;
     last = s;
