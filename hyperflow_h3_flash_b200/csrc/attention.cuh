@@ -146,6 +146,16 @@ __device__ __forceinline__ int attn_work(const AttnParams& p, const AttnPlace& a
   return max(n, 1) * attn_unit(p, a);
 }
 
+// Sum of v over the lanes up to this one.
+__device__ __forceinline__ int attn_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
 // Finds items by number; the whole warp calls find().  (base, block) is the number of the first item of the 32 sequences
 // last looked at.
 struct AttnWalk {
@@ -170,13 +180,7 @@ struct AttnWalk {
         attn_bounds(p.cu_q, b, p.Tq, q0, lq);
         attn_bounds(p.cu_k, b, p.Tk, k0, lk);
       }
-      const int mine = (lq + span - 1) / span * p.heads_kv;
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
+      const int mine = (lq + span - 1) / span * p.heads_kv, upto = attn_scan(mine, lane);
       const int rel = item - base;
       const uint32_t after = __ballot_sync(0xffffffffu, rel < upto);
       if (!after) {
@@ -223,30 +227,42 @@ struct AttnShares {
     if (lane == 0) pre[0] = 0;
 #pragma unroll 1
     for (int k = 0; k < items; k += 32) {
+      // a lane for each of 32 items, which looks its sequence up among 32 sequences at a time, held by a lane each
+      const int number = first + k + lane;
       int base = walk.base, work = 0, unit = 1;
 #pragma unroll 1
-      for (int b = walk.block; b < p.batch && base < first + items; ++b) {
+      for (int block = walk.block; block < p.batch && base < first + k + 32; block += 32) {
+        AttnPlace mine = {};
+        if (block + lane < p.batch) {
+          attn_bounds(p.cu_q, block + lane, p.Tq, mine.q0, mine.lq);
+          attn_bounds(p.cu_k, block + lane, p.Tk, mine.k0, mine.lk);
+        }
+        const int upto = attn_scan((mine.lq + span - 1) / span * p.heads_kv, lane);
+        const int rel = number - base;
+        int at = 0;  // sequences that end at or before the item
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+          const int v = __shfl_sync(0xffffffffu, upto, at + o - 1);
+          if (v <= rel) at += o;
+        }
         AttnPlace a;
-        attn_bounds(p.cu_q, b, p.Tq, a.q0, a.lq);
-        attn_bounds(p.cu_k, b, p.Tk, a.k0, a.lk);
-        const int n = (a.lq + span - 1) / span * p.heads_kv, x = first + k + lane - base;
-        if (x >= 0 && x < n) {
-          attn_place(p, x, a);
+        a.lq = __shfl_sync(0xffffffffu, mine.lq, at);
+        a.lk = __shfl_sync(0xffffffffu, mine.lk, at);
+        const int before = __shfl_sync(0xffffffffu, upto, max(at - 1, 0)), all = __shfl_sync(0xffffffffu, upto, 31);
+        if (rel >= 0 && rel < all) {
+          attn_place(p, rel - (at ? before : 0), a);
           work = attn_work(p, a);
           unit = attn_unit(p, a);
         }
-        base += n;
+        base += all;
       }
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, work, o);
-        if (lane >= o) work += v;
-      }
+      work = k + lane < items ? work : 0;
+      work = attn_scan(work, lane);
       if (k + lane < items) {
         pre[k + lane + 1] = total + work;
         units[k + lane] = static_cast<uint8_t>(unit);
       }
-      total += __shfl_sync(0xffffffffu, work, min(31, items - k - 1));
+      total += __shfl_sync(0xffffffffu, work, 31);
     }
     __syncwarp();
     // A share of less than 8 units costs more than it saves, unless it is an item of its own.  (No two edges can fall on
@@ -984,7 +1000,8 @@ __global__ void __launch_bounds__(kAtThreads, 1)
 #pragma unroll
             for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
           const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-          const bool grow = m == -CUDART_INF_F ? top != m : !((top - m) * c2 <= kRescaleLog2);
+          // (rows without a query hold what was in shared memory: they must not ask for a rescaling at every tile)
+          const bool grow = keys > 0 && (m == -CUDART_INF_F ? top != m : !((top - m) * c2 <= kRescaleLog2));
           if (!__any_sync(0xffffffffu, grow)) break;
           const float f = grow ? (m == -CUDART_INF_F ? 0.0f : exp2_approx((m - top) * c2)) : 1.0f;
           if (grow) m = fmaf(top, 0.0f, top);  // top, and NaN for +infinity: its weight is exp(inf - inf)
@@ -1200,15 +1217,19 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_con
     const int c = lane * 4;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float total = 0.0f;
-    for (int s = first; s <= last; ++s) {
-      const float z = p.part_lse[slot(s)];
-      if (z == -CUDART_INF_F) continue;
-      const float w = exp2f(z - m);
-      total += w;
-      if (c < p.D) {
-        const float4 f = *reinterpret_cast<const float4*>(p.part_o + slot(s) * p.D + c);
-        acc.x = fmaf(w, f.x, acc.x), acc.y = fmaf(w, f.y, acc.y);
-        acc.z = fmaf(w, f.z, acc.z), acc.w = fmaf(w, f.w, acc.w);
+    for (int from = first; from <= last; from += 32) {  // a lane for each part's weight, four rows in flight
+      const float z = from + lane <= last ? p.part_lse[slot(from + lane)] : -CUDART_INF_F;
+      const float mine = z == -CUDART_INF_F ? 0.0f : exp2f(z - m);
+      const int n = min(32, last - from + 1);
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const float w = __shfl_sync(0xffffffffu, mine, k);
+        total += w;
+        if (c < p.D) {  // (a part without keys holds zeros)
+          const float4 f = *reinterpret_cast<const float4*>(p.part_o + slot(from + k) * p.D + c);
+          acc.x = fmaf(w, f.x, acc.x), acc.y = fmaf(w, f.y, acc.y);
+          acc.z = fmaf(w, f.z, acc.z), acc.w = fmaf(w, f.w, acc.w);
+        }
       }
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;

@@ -178,7 +178,9 @@ int launch_attention(const DeviceState& st, const CUtensorMap& tq, const CUtenso
   kernel<<<static_cast<unsigned>(items), kAtThreads, AttnCfg<NP>::kSmemBytes, stream>>>(tq, tk, tv, p);
   if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e);
   if (p.shares > 0) {
-    attention_combine_kernel<T><<<dim3(p.shares, 4), 256, 0, stream>>>(p);
+    // a warp for each row that an item has at most (few tokens have few)
+    const int positions = p.Tq < 2 * p.positions ? p.Tq : 2 * p.positions;
+    attention_combine_kernel<T><<<dim3(p.shares, (positions * p.group + 7) / 8), 256, 0, stream>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e);
   }
   return CONVROT_OK;
