@@ -20,6 +20,7 @@ grad is refused while grad mode is on.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from collections.abc import Sequence
 
@@ -34,41 +35,53 @@ MAX_HEAD_DIM = 128  # of attention; qk_norm_rope takes heads up to 256
 
 
 def _no_grad(*tensors: Tensor | None) -> None:
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            raise ValueError("attention operators are inference only: use torch.no_grad() or detach the inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("attention operators are inference only: use torch.no_grad() or detach the inputs")
 
 
-def _call(fn: str, device: torch.device, *args) -> None:
+def _call(entry, device: torch.device, *args):
     """One library call on the tensors' device and its current stream."""
-    # (the raw stream of the allocator's bookkeeping: a torch.cuda.Stream object takes longer to make than the launch)
+    # (the raw stream: a torch.cuda.Stream object takes as long to make as the launch)
     index = device.index
-    entry = getattr(_lib.lib(), fn)
     if index == torch._C._cuda_getDevice():
-        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device):
-            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        _lib.check(rc, fn)
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(device):
+        return entry(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _heads(t: Tensor, name: str, like: Tensor | None = None) -> None:
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(t.shape)}")
-    if t.is_cuda and t.dtype not in _DTYPES:
-        raise ValueError(f"{name} must be bfloat16 or float16, got {t.dtype}")
-    if t.stride(2) != 1 and t.shape[2] != 1:
-        raise ValueError(f"{name} must be contiguous in its last dimension")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+def _heads(t: Tensor, name: str, like: Tensor | None = None) -> tuple[torch.Size, tuple[int, ...]]:
+    """Shape and strides of a [tokens, heads, head_dim] tensor, of the type and device of ``like``."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got shape {tuple(shape)}")
+    if like is None:
+        if t.dtype not in _DTYPES and t.is_cuda:
+            raise ValueError(f"{name} must be bfloat16 or float16, got {t.dtype}")
+    elif t.dtype is not like.dtype or t.device != like.device:
         raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if strides[2] != 1 and shape[2] != 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    return shape, strides
 
 
-def _new(x: Tensor) -> Tensor:
-    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+def _output(out: Tensor | None, x: Tensor, name: str) -> Tensor:
+    if out is None:
+        if x.is_contiguous():
+            return torch.empty_like(x)
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    if _heads(out, name, x)[0] != x.shape:
+        raise ValueError(f"{name} must have shape {tuple(x.shape)}, got {tuple(out.shape)}")
+    return out
 
 
 # ------------------------------------------------------------------------------------------------ positions
+
+
+@functools.lru_cache(maxsize=64)
+def _host_arrays(axes: tuple[int, ...], thetas: tuple[float, ...]):
+    return (ctypes.c_int * len(axes))(*axes), (ctypes.c_double * len(thetas))(*thetas)
 
 
 def rotary_table(positions: Tensor, axes: Sequence[int], *, theta: float | Sequence[float] = 10000.0) -> Tensor:
@@ -101,9 +114,10 @@ def rotary_table(positions: Tensor, axes: Sequence[int], *, theta: float | Seque
     if positions.stride(1) != 1 and len(axes) > 1 or positions.stride(0) < len(axes):
         positions = positions.contiguous()
     out = torch.empty(T, R // 2, 2, dtype=torch.float32, device=positions.device)
-    _call("convrot_rotary_table", positions.device, positions.data_ptr(), _POSITIONS[positions.dtype],
-          max(positions.stride(0), len(axes)), T, len(axes), (ctypes.c_int * len(axes))(*axes),
-          (ctypes.c_double * len(axes))(*thetas), out.data_ptr())
+    rc = _call(_lib.lib().convrot_rotary_table, positions.device, positions.data_ptr(), _POSITIONS[positions.dtype],
+               max(positions.stride(0), len(axes)), T, len(axes), *_host_arrays(axes, tuple(thetas)), out.data_ptr())
+    if rc:
+        _lib.check(rc, "convrot_rotary_table")
     return out
 
 
@@ -131,13 +145,12 @@ def _norm_rope_torch(x: Tensor, weight: Tensor | None, eps: float, norm: bool, t
     return y.to(x.dtype)
 
 
-def _rope_out(out: Tensor | None, x: Tensor, name: str) -> Tensor:
-    if out is None:
-        return _new(x)
-    _heads(out, name, x)
-    if out.shape != x.shape:
-        raise ValueError(f"{name} must have shape {tuple(x.shape)}, got {tuple(out.shape)}")
-    return out
+def _weight(w: Tensor, D: int, q: Tensor) -> bool:
+    """Whether a norm weight is fp32 (else it is of q's type)."""
+    f32 = w.dtype is torch.float32
+    if w.shape != (D,) or not (f32 or w.dtype is q.dtype) or w.device != q.device or not w.is_contiguous():
+        raise ValueError(f"norm weights must be contiguous [{D}] of {q.dtype} or float32 on {q.device}")
+    return f32
 
 
 def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None = None, k_weight: Tensor | None = None,
@@ -150,35 +163,37 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
     (``rotary_table``'s, fp32 ``[T, R / 2, 2]``; None: no rotation): pairs of neighbours if ``interleaved``, else
     ``(j, j + R / 2)``.  fp32 arithmetic, one rounding.  Returns the new q (and k when given).  ``q_out`` / ``k_out`` may
     be the inputs themselves; an output that overlaps an input in any other way is not supported."""
-    if torch.is_grad_enabled():
-        _no_grad(q, k, q_weight, k_weight)
-    _heads(q, "q")
+    _no_grad(q, k, q_weight, k_weight)
+    (T, Hq, D), qs = _heads(q, "q")
     if k is not None:
-        _heads(k, "k", q)
-        if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-            raise ValueError(f"k must have q's tokens and head_dim, got {tuple(k.shape)} beside {tuple(q.shape)}")
+        k_shape, ks = _heads(k, "k", q)
+        if k_shape[0] != T or k_shape[2] != D:
+            raise ValueError(f"k must have q's tokens and head_dim, got {tuple(k_shape)} beside {tuple(q.shape)}")
     elif k_weight is not None or k_out is not None:
         raise ValueError("k_weight and k_out need k")
-    T, _, D = q.shape
-    if not norm and table is None:
-        raise ValueError("nothing to do: norm=False and no table")
-    if not norm and (q_weight is not None or k_weight is not None):
-        raise ValueError("norm weights need norm=True")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        if w.shape != (D,) or w.device != q.device or w.dtype not in (q.dtype, torch.float32) or not w.is_contiguous():
-            raise ValueError(f"norm weights must be contiguous [{D}] of {q.dtype} or float32 on {q.device}")
-        if w.dtype != weights[0].dtype:
+    f32 = None
+    if q_weight is not None:
+        f32 = _weight(q_weight, D, q)
+    if k_weight is not None:
+        k_f32 = _weight(k_weight, D, q)
+        if f32 is not None and f32 != k_f32:
             raise ValueError("q_weight and k_weight must have one type")
-    if not (eps >= 0 and math.isfinite(eps)):
+        f32 = k_f32
+    if not norm:
+        if table is None:
+            raise ValueError("nothing to do: norm=False and no table")
+        if f32 is not None:
+            raise ValueError("norm weights need norm=True")
+    if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     R = 0
     if table is not None:
-        if table.dim() != 3 or table.shape[0] != T or table.shape[2] != 2 or table.dtype != torch.float32 or \
+        shape = table.shape
+        if len(shape) != 3 or shape[0] != T or shape[2] != 2 or table.dtype is not torch.float32 or \
                 table.device != q.device:
-            raise ValueError(f"table must be float32 [{T}, R / 2, 2] on {q.device}, got {table.dtype} "
-                             f"{tuple(table.shape)} on {table.device}")
-        R = 2 * table.shape[1]
+            raise ValueError(f"table must be float32 [{T}, R / 2, 2] on {q.device}, got {table.dtype} {tuple(shape)} on "
+                             f"{table.device}")
+        R = 2 * shape[1]
         if R > D or R % (8 if interleaved else 16) or R == 0:
             raise ValueError(f"the table rotates {R} channels: must be a multiple of {8 if interleaved else 16} up to "
                              f"head_dim {D}")
@@ -186,29 +201,31 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
             table = table.contiguous()
     if not q.is_cuda:
         qo = _norm_rope_torch(q, q_weight, eps, norm, table, interleaved)
-        qo = qo if q_out is None else _rope_out(q_out, q, "q_out").copy_(qo)
+        qo = qo if q_out is None else _output(q_out, q, "q_out").copy_(qo)
         if k is None:
             return qo
         ko = _norm_rope_torch(k, k_weight, eps, norm, table, interleaved)
-        return qo, (ko if k_out is None else _rope_out(k_out, k, "k_out").copy_(ko))
+        return qo, (ko if k_out is None else _output(k_out, k, "k_out").copy_(ko))
     if D % 8 or not 8 <= D <= 256:
         raise ValueError(f"head_dim must be a multiple of 8 up to 256, got {D}")
-    qo = _rope_out(q_out, q, "q_out")
-    ko = None if k is None else _rope_out(k_out, k, "k_out")
-    if k is not None and T and (qo.data_ptr() in (k.data_ptr(), ko.data_ptr()) or ko.data_ptr() == q.data_ptr()):
-        raise ValueError("q_out and k_out must not be the other's input or each other")
-    if q.shape[1] == 0 or (k is not None and k.shape[1] == 0):
+    if Hq == 0 or (k is not None and k_shape[1] == 0):
         raise ValueError("q and k need at least one head")
-    qs, qos = q.stride(), qo.stride()
+    qo = _output(q_out, q, "q_out")
+    qos, q_ptr, qo_ptr = qo.stride(), q.data_ptr(), qo.data_ptr()
     if k is None:
-        kk = (None, 0, 0, None, 0, 0, 0)
+        ko, kk = None, (None, 0, 0, None, 0, 0, 0)
     else:
-        ks, kos = k.stride(), ko.stride()
-        kk = (k.data_ptr(), ks[0], ks[1], ko.data_ptr(), kos[0], kos[1], k.shape[1])
-    _call("convrot_qk_norm_rope", q.device, q.data_ptr(), qs[0], qs[1], qo.data_ptr(), qos[0], qos[1], q.shape[1], *kk, T,
-          D, _DTYPES[q.dtype], norm, None if q_weight is None else q_weight.data_ptr(),
-          None if k_weight is None else k_weight.data_ptr(), bool(weights) and weights[0].dtype == torch.float32, eps,
-          None if table is None else table.data_ptr(), R // 2, R, interleaved)
+        ko = _output(k_out, k, "k_out")
+        kos, k_ptr, ko_ptr = ko.stride(), k.data_ptr(), ko.data_ptr()
+        if T and (qo_ptr == k_ptr or qo_ptr == ko_ptr or ko_ptr == q_ptr):
+            raise ValueError("q_out and k_out must not be the other's input or each other")
+        kk = (k_ptr, ks[0], ks[1], ko_ptr, kos[0], kos[1], k_shape[1])
+    rc = _call(_lib.lib().convrot_qk_norm_rope, q.device, q_ptr, qs[0], qs[1], qo_ptr, qos[0], qos[1], Hq, *kk, T, D,
+               _DTYPES[q.dtype], norm, None if q_weight is None else q_weight.data_ptr(),
+               None if k_weight is None else k_weight.data_ptr(), f32 is True, eps,
+               None if table is None else table.data_ptr(), R // 2, R, interleaved)
+    if rc:
+        _lib.check(rc, "convrot_qk_norm_rope")
     return qo if k is None else (qo, ko)
 
 
@@ -251,14 +268,11 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
 
     Scores, statistics and sums are fp32; the weights are rounded to the inputs' type for their product with v.  Few
     queries over long keys are split over the GPU and joined in a fixed order: results do not vary from run to run."""
-    if torch.is_grad_enabled():
-        _no_grad(q, k, v)
-    _heads(q, "q")
-    _heads(k, "k", q)
-    _heads(v, "v", q)
-    Tq, Hq, D = q.shape
-    Tk, Hkv, _ = k.shape
-    if v.shape != k.shape or k.shape[2] != D:
+    _no_grad(q, k, v)
+    (Tq, Hq, D), qs = _heads(q, "q")
+    (Tk, Hkv, Dk), ks = _heads(k, "k", q)
+    v_shape, vs = _heads(v, "v", q)
+    if Dk != D or v_shape != k.shape:
         raise ValueError(f"k and v must be [Tk, Hkv, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
     if Hkv == 0 or Hq == 0 or Hq % Hkv or Hq // Hkv > 128:
         raise ValueError(f"{Hq} query heads cannot share {Hkv} key heads (at most 128 each)")
@@ -278,12 +292,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
         if cu_q.shape != cu_k.shape:
             raise ValueError(f"cu_q and cu_k must have one length, got {cu_q.shape[0]} and {cu_k.shape[0]}")
         batch = cu_q.shape[0] - 1
-    if out is None:
-        out = _new(q)
-    else:
-        _heads(out, "out", q)
-        if out.shape != q.shape:
-            raise ValueError(f"out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    out = _output(out, q, "out")
     lse = torch.empty(Tq, Hq, dtype=torch.float32, device=q.device) if return_lse else None
     if not q.is_cuda:
         _attention_torch(q, k, v, cu_q, cu_k, causal, scale, out, lse)
@@ -298,11 +307,13 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
         raise ValueError(f"attention does not take {Tq} queries and {Tk} keys in {batch} sequences of {Hq} heads")
     # from torch's stream-ordered allocator: freed at return, reused only by later work of this stream (or graph)
     space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-    _call("convrot_attention", device, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-          None if cu_q is None else cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(), batch, Tq, Tk, Hq, Hkv, D,
-          _DTYPES[q.dtype], scale, causal, out.data_ptr(), os[0], os[1], None if lse is None else lse.data_ptr(),
-          None if space is None else space.data_ptr(), size)
+    os = out.stride()
+    rc = _call(handle.convrot_attention, device, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+               vs[0], vs[1], None if cu_q is None else cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(), batch,
+               Tq, Tk, Hq, Hkv, D, _DTYPES[q.dtype], scale, causal, out.data_ptr(), os[0], os[1],
+               None if lse is None else lse.data_ptr(), None if space is None else space.data_ptr(), size)
+    if rc:
+        _lib.check(rc, "convrot_attention")
     return out if lse is None else (out, lse)
 
 

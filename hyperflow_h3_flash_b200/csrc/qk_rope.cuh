@@ -142,7 +142,7 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
 // costs two operations an element beside its sum of squares and the scale.  (Every row with its own weight and rotation
 // took 350 us for 32760 tokens x 2 x 40 heads of 128, bound by issue slots.)  With pairs of neighbours a lane holds 8
 // channels; with pairs R / 2 apart it holds the 8 channels and their partners, R / 2 further (by shuffles from the
-// partners' lane they cost 306 us instead of 248), and lanes behind the rotated part hold 16 channels in a row.
+// partners' lane they cost 306 us instead of 239), and lanes behind the rotated part hold 16 channels in a row.
 template <class T, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __grid_constant__ QkRopeParams p) {
   constexpr int CH = INTERLEAVED ? 1 : 2;  // 8-channel pieces of a lane
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __g
     for (int h = 0; h < CH; ++h) {
       raw[r][h] = make_uint4(0, 0, 0, 0);
       if (here[h] && row0 + r * per < heads)
-        raw[r][h] = *reinterpret_cast<const uint4*>(in + r * per * in_h + h * apart);
+        raw[r][h] = __ldcs(reinterpret_cast<const uint4*>(in + r * per * in_h + h * apart));
     }
 
   // out[i] = mine[i] x[i] + other[i] x[i's partner]
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __g
         u.y = Pack16<T>::pack(y[8 * h + 2], y[8 * h + 3]);
         u.z = Pack16<T>::pack(y[8 * h + 4], y[8 * h + 5]);
         u.w = Pack16<T>::pack(y[8 * h + 6], y[8 * h + 7]);
-        *reinterpret_cast<uint4*>(out + r * per * out_h + h * apart) = u;
+        __stcs(reinterpret_cast<uint4*>(out + r * per * out_h + h * apart), u);
       }
   }
 }
