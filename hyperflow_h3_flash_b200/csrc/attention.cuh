@@ -59,9 +59,11 @@ struct AttnParams {
   const int32_t* cu_k;
   int batch, Tq, Tk;
   int heads_kv, group, D;
-  int positions;  // query positions in a 128-row tile: 128 / group
+  int positions;      // query positions in a 128-row tile: 128 / group
+  int group_inverse;  // 65536 / group, rounded up: exact for the quotient of a row below 128
   float scale_log2;
   int causal;
+  int head_block;  // key heads whose items follow each other by query tile
   void* out;
   int64_t out_t, out_h;
   float* lse;  // [Tq, heads] or null
@@ -132,8 +134,11 @@ __device__ __forceinline__ int attn_tiles(const AttnParams& p, const AttnPlace& 
 __device__ __forceinline__ void attn_place(const AttnParams& p, int local, AttnPlace& a) {
   const int span = 2 * p.positions;
   const int nq = (a.lq + span - 1) / span;
-  a.head = local / nq;
-  const int qt = local - a.head * nq;
+  // blocks of `head_block` heads; in a block by query tile, and for each by head
+  const int block = local / (nq * p.head_block), in_block = local - block * nq * p.head_block;
+  const int heads = min(p.head_block, p.heads_kv - block * p.head_block);
+  const int qt = heads == 1 ? in_block : in_block / heads;
+  a.head = block * p.head_block + in_block - qt * heads;
   a.pos = (p.causal ? nq - 1 - qt : qt) * span;
 }
 
@@ -281,7 +286,8 @@ struct AttnShares {
     return from + (x - from + unit - 1) / unit * unit;
   }
   __device__ __forceinline__ int place(int s) const {  // before it is moved to a step
-    return static_cast<int>(static_cast<int64_t>(total) * s / shares);
+    const int q = total / shares;  // total * s / shares, without its 64-bit product
+    return q * s + (total - q * shares) * s / shares;
   }
   __device__ __forceinline__ int edge(int s, int lane) const {
     if (s >= shares) return total;
@@ -927,7 +933,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       const int n = uniform(item->nt[i]);
       // (registers are short below: what only the output needs is worked out again there)
       auto position = [&](bool& valid) {
-        const int in_tile = row / p.group;
+        const int in_tile = row * p.group_inverse >> 16;  // row / group
         const int pos = (twin ? 0 : i * p.positions) + in_tile;
         valid = in_tile < p.positions && pos < item->left;
         return pos;
@@ -981,6 +987,16 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         // The first half of the weights is taken with the maximum so far, while the tile's own maximum is still being
         // found: it seldom grows enough to matter, and then the half is taken again.  Finding the maximum first would
         // leave the special-function unit idle meanwhile.
+        if (j == 0) {  // the first tile goes by the maximum of its first 32 scores
+          float mx[2] = {m, m};
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            mx[0] = max3(mx[0], __uint_as_float(s[0][e]), __uint_as_float(s[0][e + 1]));
+            mx[1] = max3(mx[1], __uint_as_float(s[0][e + 2]), __uint_as_float(s[0][e + 3]));
+          }
+          m = max3(mx[0], mx[1], mx[1]);
+          m = m == -CUDART_INF_F ? m : fmaf(m, 0.0f, m);
+        }
         uint64_t sum[2];
         float neg;
 #pragma unroll 1
@@ -1067,21 +1083,21 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         }
       }
       if (warp_valid) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees no key gives zeros
+        const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);  // a row that sees no key gives zeros
         w0 *= inv;
         w1 *= inv;
         const bool parts = uniform(item->part) >= 0, any = n > 0 && inv != 0.0f;
         int r = row;
         asm volatile("" : "+r"(r));  // not kept from before
-        const int in_tile = r / p.group;
+        const int in_tile = r * p.group_inverse >> 16;
         const int64_t t = item->q_row + (twin ? 0 : i * p.positions) + in_tile;
         const int head = item->head * p.group + r - in_tile * p.group;
         const int64_t part = static_cast<int64_t>(item->part) * 256 + i * 128 + row;
-        if (valid) {
+        if (valid && (parts || p.lse)) {
           const float lse2 = l == 0.0f ? -CUDART_INF_F : fmaf(m, c2, log2f(l));
           if (parts)
             p.part_lse[part] = lse2;
-          else if (p.lse)
+          else
             p.lse[t * (p.heads_kv * p.group) + head] = lse2 * 0.69314718055994530942f;
         }
         // Rows go out through the warp's staging buffer, 128 bytes of 32 rows at a time, so that eight lanes write 128
@@ -1189,7 +1205,7 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_con
   if (!walk.find(p, whole + x, lane, a)) return;
   const int unit = attn_unit(p, a);
   // the edges that lie inside this item
-  int s = max(1, static_cast<int>((static_cast<int64_t>(from) * shares + sh.total - 1) / max(sh.total, 1)));
+  int s = max(1, static_cast<int>(static_cast<int64_t>(from) * shares / max(sh.total, 1)));
   int first = 0, last = -1;  // shares of the item, if it was divided
   for (; s < shares && sh.place(s) < upto; ++s) {
     const int e = sh.snap(sh.place(s), from, upto, unit);

@@ -229,8 +229,14 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
   p.group = heads_q / heads_kv;
   p.D = D;
   p.positions = kAtTile / p.group;
+  p.group_inverse = (65536 + p.group - 1) / p.group;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.causal = causal ? 1 : 0;
+  // Causal items go out longest first; over as many heads at once as keep their keys and values in L2, so that the
+  // last ones are short.
+  const int64_t head_bytes = (Tk + batch - 1) / batch * D * 4 + 1;
+  const int64_t block = (int64_t{96} << 20) / head_bytes;
+  p.head_block = !causal || block < 1 ? 1 : block < heads_kv ? static_cast<int>(block) : heads_kv;
   p.out = out;
   p.out_t = out_t;
   p.out_h = out_h;
