@@ -37,10 +37,12 @@ namespace convrot {
 constexpr int kAtTile = 128;
 constexpr int kAtThreads = 384;
 constexpr int kAtPanelBytes = 128 * 128;  // 128 rows x 64 channels of 16 bits, 128-byte swizzled rows
+constexpr uint64_t kDrainNs = 1000000000ull;  // for work of its own that a CTA that gave up has still in flight
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kFirstSteps = 6;  // 16-key steps of a tile's weights that are handed over before the rest
 
 constexpr int kItems = 4;        // items on their way through the CTA
+constexpr int kBadWords = 13;     // of an item: any, and a bit for each key of the (at most 3) tiles seen in part
 constexpr int kMaxShares = 192;  // most CTAs that share the last items evenly
 
 template <int NP>
@@ -49,7 +51,7 @@ struct AttnCfg {  // NP: 64-channel panels of a head (1: D <= 64, 2: D <= 128)
   static constexpr int kStages = NP == 2 ? 4 : 8;
   static constexpr int kStageOut = 4096;  // output staging of a warp: 32 rows of 128 bytes
   static constexpr int kNumBars = 2 * kStages + 19 + 3 * kItems;
-  static constexpr int kSmallBytes = 8 * kNumBars + kItems * 48 + 2 * 16 + 5 * kMaxShares + 4 + 16;
+  static constexpr int kSmallBytes = 8 * kNumBars + kItems * 48 + 2 * 16 + 5 * kMaxShares + 4 + 16 + 4 * kItems * kBadWords;
   static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 8 * kStageOut + kSmallBytes + 1024;
   static constexpr int kO = 256;  // TMEM columns from S_i to O_i
 };
@@ -64,6 +66,8 @@ struct AttnParams {
   float scale_log2;
   int causal;
   int head_block;  // key heads whose items follow each other by query tile
+  const void* v;  // (the kernel's loads go through the tensor maps)
+  int64_t v_t, v_h;
   void* out;
   int64_t out_t, out_h;
   float* lse;  // [Tq, heads] or null
@@ -100,7 +104,7 @@ struct AttnItem {
   int see;          // keys from k_row that the first position sees (position r: r more, if causal)
   int nt[2];        // key tiles of each query tile
   int twin;         // tile 1 is tile 0 again
-  int fixing;       // the last value tile has rows of another sequence
+  int check;        // first key tile whose values have to be looked at (see warp 10)
   int part;         // slot of the partial result, or -1
   int valid;        // 0: no more work
 };
@@ -528,7 +532,7 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], float c2, float
 
 // ------------------------------------------------------------------------------------------------ the kernel
 
-template <class T, int NP>
+template <class T, int NP, bool CAUSAL>
 __global__ void __launch_bounds__(kAtThreads, 1)
     attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ AttnParams p) {
@@ -548,6 +552,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   uint8_t* units = reinterpret_cast<uint8_t*>(pre + kMaxShares + 1);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(units + kMaxShares);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  uint32_t* bad = tmem_holder + 4;
   const uint32_t bar0 = smem_u32(bars);
   auto kv_full = [&](int s) { return bar0 + 8 * s; };
   auto kv_empty = [&](int s) { return bar0 + 8 * (S + s); };
@@ -612,7 +617,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
     const int4 x = src[0], y = src[1], z = src[2];
     it.q_row = uniform(x.x), it.left = uniform(x.y), it.k_row = uniform(x.z), it.keys = uniform(x.w);
     it.head = uniform(y.x), it.see = uniform(y.y), it.nt[0] = uniform(y.z), it.nt[1] = uniform(y.w);
-    it.twin = uniform(z.x), it.fixing = uniform(z.y), it.part = uniform(z.z), it.valid = uniform(z.w);
+    it.twin = uniform(z.x), it.check = uniform(z.y), it.part = uniform(z.z), it.valid = uniform(z.w);
     release();
   };
 
@@ -637,7 +642,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
           int4* dst = reinterpret_cast<int4*>(item_smem + at);
           dst[0] = make_int4(x.q_row, x.left, x.k_row, x.keys);
           dst[1] = make_int4(x.head, x.see, x.nt[0], x.nt[1]);
-          dst[2] = make_int4(x.twin, x.fixing, x.part, x.valid);
+          dst[2] = make_int4(x.twin, x.check, x.part, x.valid);
           bar_arrive(item_full(at));  // releases the stores above
         }
         __syncwarp();
@@ -691,7 +696,9 @@ __global__ void __launch_bounds__(kAtThreads, 1)
           it.nt[1] = max(min(n1, hi) - lo, 0);
           it.twin = it.left <= p.positions && it.nt[0] > 1;
           const int n = max(it.nt[0], it.nt[1]);
-          it.fixing = n > 0 && n * kAtTile > it.keys && a.k0 + a.lk < p.Tk;
+          // the last tile if rows behind it are another's, and the tiles that the first position does not see whole
+          it.check = n > 0 && n * kAtTile > it.keys && a.k0 + a.lk < p.Tk ? n - 1 : n;
+          if (p.causal) it.check = min(it.check, max(it.see, 0) / kAtTile);
           if (it.twin) {
             it.nt[1] = n / 2;
             it.nt[0] = n - it.nt[1];
@@ -772,9 +779,9 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       if (guard.aborted() && lane == 0) {  // let every load this thread issued land before the CTA leaves
         volatile int never = 0;
         for (int s = 0; s < S; ++s)
-          if (issued_mask >> s & 1) mbar_wait_bounded(bars + s, issued_parity >> s & 1, p.wait_limit_ns, &never);
+          if (issued_mask >> s & 1) mbar_wait_bounded(bars + s, issued_parity >> s & 1, kDrainNs, &never);
         for (int i = 0; i < 2; ++i)
-          if (q_count[i]) mbar_wait_bounded(bars + 2 * S + i, (q_count[i] - 1) & 1, p.wait_limit_ns, &never);
+          if (q_count[i]) mbar_wait_bounded(bars + 2 * S + i, (q_count[i] - 1) & 1, kDrainNs, &never);
       }
     } else if (warp == 8) {
       // -------------------------------------------------------------- MMA issuer
@@ -832,6 +839,13 @@ __global__ void __launch_bounds__(kAtThreads, 1)
           }
           __syncwarp();
         }
+        // Warp 10 looks at the values of the tiles from `check` on, one tile ahead of their use (they are the next load).
+        auto look = [&](int tile) {
+          if (tile < it.check || tile >= (twin ? all : n)) return;
+          guard.wait(kv_full(slot), slot_phase);
+          if (lane == 0) bar_arrive(v_need);
+        };
+        look(0);
 #pragma unroll 1
         for (int step = 0; step < 2 * n; ++step) {
           const int i = step & 1, j = step >> 1, mine = i == 0 ? it.nt[0] : it.nt[1], q = twin ? 0 : i;
@@ -847,9 +861,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
             } else {
               guard.wait(kv_full(vs), vph);
             }
-            // cleared by warp 10 while the softmax still works on this tile
-            if (it.fixing && tile + 1 == (twin ? all : n)) {
-              if (lane == 0) bar_arrive(v_need);
+            if (tile >= it.check) {
               guard.wait(v_fixed, fixes & 1);
               ++fixes;
             }
@@ -887,37 +899,87 @@ __global__ void __launch_bounds__(kAtThreads, 1)
             }
           }
           __syncwarp();
+          if (i == 1 || twin) look(tile + 1);
         }
       }
       if (guard.aborted()) {  // the products still in flight read shared memory and TMEM
         volatile int never = 0;
         if (elect_one()) bar_commit(drain);
         __syncwarp();
-        mbar_wait_bounded(bars + 2 * S + 14, 0, p.wait_limit_ns, &never);
+        mbar_wait_bounded(bars + 2 * S + 14, 0, kDrainNs, &never);
       }
     } else if (warp == 10) {
-      // -------------------------------------------------------------- value rows behind a sequence's end
-      // Their weights are exactly zero, but 0 * NaN is not: another request's rows must not reach this one.  (Rows
-      // behind the tensor's end are zeros that TMA filled in.)
+      // -------------------------------------------------------------- values that a row of the tile must not meet
+      // A weight of zero does not keep a NaN or an infinity out of a product.  Rows behind a sequence's end (another
+      // request's) are cleared.  In the tiles that causal rows see in part, values that are not finite are cleared and
+      // their keys noted: the rows that do see them get those values with the output.  (Rows behind the tensor's end are zeros
+      // that TMA filled in.)
       uint32_t slot = 0, fixes = 0;
       while (next_item()) {
+        uint32_t* noted = bad + (item_count % kItems) * kBadWords;
         copy_item();
         const int n = it.twin ? it.nt[0] + it.nt[1] : max(it.nt[0], it.nt[1]);
-        if (n == 0) continue;
-        const uint32_t at = (slot + 2 * n - 1) % S;  // the last value tile is the item's last load
+        if (it.check < n && lane < kBadWords) noted[lane] = 0;
+        __syncwarp();
+#pragma unroll 1
+        for (int t = it.check; t < n; ++t) {
+          const uint32_t load = it.twin ? min(2 * t + 2, 2 * n - 1) : 2 * t + 1;  // its number among the item's loads
+          uint8_t* tile = ring + (slot + load) % S * Cfg::kTileBytes;
+          guard.wait(v_need, fixes & 1);
+          ++fixes;
+          __syncwarp();
+          const int rows = min(it.keys - t * kAtTile, kAtTile);
+          if (rows < kAtTile)
+            for (int c = 0; c < NP; ++c)
+              for (int r = rows * 8 + lane; r < kAtTile * 8; r += 32)
+                *reinterpret_cast<uint4*>(tile + c * kAtPanelBytes + r * 16) = make_uint4(0, 0, 0, 0);
+          if (CAUSAL) {
+            // 0 * x is NaN for what is not finite; two values to an instruction, several loads in flight
+            using T2 = typename Pack16<T>::Two;
+            const T2 zero = Pack16<T>::both(0.0f);
+            T2 sum[2] = {zero, zero};
+#pragma unroll 1
+            for (int c = 0; c < NP; ++c) {
+#pragma unroll 8
+              for (int r = 0; r < kAtTile; r += 4) {  // 8 lanes for each of 4 rows (rows behind the end are zeros by now)
+                const uint4 v = *reinterpret_cast<const uint4*>(tile + c * kAtPanelBytes + r * 128 + lane * 16);
+                sum[0] = __hfma2(*reinterpret_cast<const T2*>(&v.x), zero, sum[0]);
+                sum[1] = __hfma2(*reinterpret_cast<const T2*>(&v.y), zero, sum[1]);
+                sum[0] = __hfma2(*reinterpret_cast<const T2*>(&v.z), zero, sum[0]);
+                sum[1] = __hfma2(*reinterpret_cast<const T2*>(&v.w), zero, sum[1]);
+              }
+            }
+            const T2 all = __hadd2(sum[0], sum[1]);
+            if (__any_sync(0xffffffffu, !__hbeq2(all, zero))) {
+              constexpr uint32_t kExp = kBf16 ? 0x7f807f80u : 0x7c007c00u;
+#pragma unroll 1
+              for (int r = 0; r < rows; r += 4) {
+                uint32_t hit = 0;
+#pragma unroll 1
+                for (int c = 0; c < NP; ++c) {
+                  uint32_t* at = reinterpret_cast<uint32_t*>(tile + c * kAtPanelBytes + r * 128 + lane * 16);
+#pragma unroll 1
+                  for (int k = 0; k < 4; ++k) {
+                    const uint32_t m = __vcmpeq2(at[k] & kExp, kExp);
+                    at[k] &= ~m;
+                    hit |= m;
+                  }
+                }
+                const uint32_t which = __ballot_sync(0xffffffffu, hit != 0);
+                if (which && lane == 0) {
+                  uint32_t rows4 = 0;
+                  for (int k = 0; k < 4; ++k) rows4 |= (which >> 8 * k & 0xff) ? 1u << k : 0u;
+                  noted[1 + (t - it.check) * 4 + r / 32] |= rows4 << (r & 31);
+                  noted[0] = 1;
+                }
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) bar_arrive(v_fixed);
+        }
         slot = (slot + 2 * n) % S;
-        if (!it.fixing) continue;
-        const int rows = it.keys - (n - 1) * kAtTile;
-        guard.wait(v_need, fixes & 1);
-        ++fixes;
-        __syncwarp();
-        for (int c = 0; c < NP; ++c)
-          for (int r = rows * 8 + lane; r < kAtTile * 8; r += 32)
-            *reinterpret_cast<uint4*>(ring + at * Cfg::kTileBytes + c * kAtPanelBytes + r * 16) =
-                make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) bar_arrive(v_fixed);
       }
     }
   } else {
@@ -927,6 +989,8 @@ __global__ void __launch_bounds__(kAtThreads, 1)
     const int row = (warp & 3) * 32 + lane;
     const uint32_t s_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + i * 128;
     const float c2 = p.scale_log2;
+    // fp16 weights are taken times 2^7 (at most 2^15 with the lazy maximum): more of the small ones stay normal numbers
+    constexpr float kShift = kBf16 ? 0.0f : 7.0f;
     uint32_t s_phase = 0, o_phase = 0, twin_phase = 0;
     while (next_item()) {
       const bool twin = uniform(item->twin) != 0;
@@ -940,7 +1004,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       };
       bool valid;
       const int pos = position(valid);
-      const int keys = !valid ? 0 : (p.causal ? min(item->keys, item->see + pos) : item->keys);
+      const int keys = !valid ? 0 : (CAUSAL ? min(item->keys, item->see + pos) : item->keys);
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       // tiles before this one need no mask in any row of the warp
       const int full = __reduce_min_sync(0xffffffffu, valid ? max(keys, 0) : 0x7fffffff) / kAtTile;
@@ -1001,7 +1065,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         float neg;
 #pragma unroll 1
         for (bool again = false;; again = true) {
-          neg = m == -CUDART_INF_F ? 0.0f : -m * c2;
+          neg = m == -CUDART_INF_F ? 0.0f : fmaf(-m, c2, kShift);
           sum[0] = sum[1] = 0;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -1094,7 +1158,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         const int head = item->head * p.group + r - in_tile * p.group;
         const int64_t part = static_cast<int64_t>(item->part) * 256 + i * 128 + row;
         if (valid && (parts || p.lse)) {
-          const float lse2 = l == 0.0f ? -CUDART_INF_F : fmaf(m, c2, log2f(l));
+          const float lse2 = l == 0.0f ? -CUDART_INF_F : fmaf(m, c2, log2f(l) - kShift);
           if (parts)
             p.part_lse[part] = lse2;
           else
@@ -1169,6 +1233,35 @@ __global__ void __launch_bounds__(kAtThreads, 1)
             if (!(c & 1)) continue;
           }
           write_out((parts ? c : c >> 1) * 128);
+        }
+        if (CAUSAL) {  // values that are not finite, in tiles that rows see in part: seldom more than this look
+          const volatile uint32_t* noted = bad + (item_count % kItems) * kBadWords;
+          if (item->check < (item->twin ? item->nt[0] + item->nt[1] : max(item->nt[0], item->nt[1])) && noted[0]) {
+            // (everything worked out again: nothing is kept in registers for this)
+            int r = row;
+            asm volatile("" : "+r"(r));
+            const int in_tile = r * p.group_inverse >> 16, pos = (item->twin ? 0 : i * p.positions) + in_tile;
+            const int limit = in_tile < p.positions && pos < item->left ? min(item->keys, item->see + pos) : 0;
+            const int slot = item->part;
+            T* to = static_cast<T*>(p.out) + static_cast<int64_t>(item->q_row + pos) * p.out_t +
+                    (item->head * p.group + r - in_tile * p.group) * p.out_h;
+            float* part_to = p.part_o + (static_cast<int64_t>(slot) * 256 + i * 128 + r) * p.D;
+#pragma unroll 1
+            for (int k = 0; k < 32 * (kBadWords - 1); ++k) {
+              const int key = item->check * kAtTile + k;
+              if (!(noted[1 + k / 32] >> (k & 31) & 1) || key >= limit) continue;
+              const T* v = static_cast<const T*>(p.v) + (item->k_row + key) * p.v_t + item->head * p.v_h;
+#pragma unroll 1
+              for (int d = 0; d < p.D; ++d) {
+                const float x = static_cast<float>(v[d]);
+                if (isfinite(x)) continue;
+                if (slot >= 0)
+                  part_to[d] += x;
+                else
+                  to[d] = static_cast<T>(static_cast<float>(to[d]) + x);
+              }
+            }
+          }
         }
       }
       if (twin) {

@@ -60,6 +60,10 @@ int qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t q
   }
   if (rows == 0) return CONVROT_OK;
   if (!q || !q_out || (heads_k > 0 && (!k || !k_out))) return CONVROT_ERR_ARG;
+  // a stride of a dimension of one element does not matter
+  if (rows == 1) q_t = qo_t = k_t = ko_t = 0;
+  if (heads_q == 1) q_h = qo_h = 0;
+  if (heads_k == 1) k_h = ko_h = 0;
   const int64_t strides[] = {q_t, q_h, qo_t, qo_h, k_t, k_h, ko_t, ko_h};
   for (int i = 0; i < (heads_k ? 8 : 4); ++i) {
     if (strides[i] < 0) return CONVROT_ERR_SHAPE;
@@ -162,10 +166,10 @@ int attn_map(CUtensorMap* map, const void* base, int dtype, int D, int64_t heads
   return CONVROT_OK;
 }
 
-template <class T, int NP>
+template <class T, int NP, bool CAUSAL>
 int launch_attention(const DeviceState& st, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                      const AttnParams& p, int64_t items, cudaStream_t stream) {
-  auto kernel = attention_kernel<T, NP>;
+  auto kernel = attention_kernel<T, NP, CAUSAL>;
   int ready = -1;
   int rc = cached_resident(reinterpret_cast<const void*>(kernel), &ready);
   if (rc) return rc;
@@ -196,6 +200,12 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
   if ((cu_q == nullptr) != (cu_k == nullptr) || (!cu_q && batch != 1)) return CONVROT_ERR_ARG;
   if (Tq == 0 || batch == 0) return CONVROT_OK;
   if (!q || !out || (Tk > 0 && (!k || !v))) return CONVROT_ERR_ARG;
+  // a stride of a dimension of one element does not matter
+  const int64_t any = 128;
+  if (heads_q == 1) q_h = out_h = any;
+  if (heads_kv == 1) k_h = v_h = any;
+  if (Tq <= 1) q_t = out_t = any;
+  if (Tk <= 1) k_t = v_t = any;
   const struct {
     const void* base;
     int64_t t, h, heads, rows;
@@ -237,6 +247,9 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
   const int64_t head_bytes = (Tk + batch - 1) / batch * D * 4 + 1;
   const int64_t block = (int64_t{96} << 20) / head_bytes;
   p.head_block = !causal || block < 1 ? 1 : block < heads_kv ? static_cast<int>(block) : heads_kv;
+  p.v = v;
+  p.v_t = v_t;
+  p.v_h = v_h;
   p.out = out;
   p.out_t = out_t;
   p.out_h = out_h;
@@ -255,9 +268,13 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
   // An upper bound of the work items (the kernel finds their number; what is beyond it finds nothing).
   const int64_t items = attn_items(Tq, batch, heads_q, heads_kv) + p.shares;
   if (items > INT32_MAX / 2) return CONVROT_ERR_SHAPE;
-  if (dtype == 0)
-    return D <= 64 ? launch_attention<__nv_bfloat16, 1>(*st, tq, tk, tv, p, items, stream)
-                   : launch_attention<__nv_bfloat16, 2>(*st, tq, tk, tv, p, items, stream);
-  return D <= 64 ? launch_attention<__half, 1>(*st, tq, tk, tv, p, items, stream)
-                 : launch_attention<__half, 2>(*st, tq, tk, tv, p, items, stream);
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    if (D <= 64)
+      return causal ? launch_attention<T, 1, true>(*st, tq, tk, tv, p, items, stream)
+                    : launch_attention<T, 1, false>(*st, tq, tk, tv, p, items, stream);
+    return causal ? launch_attention<T, 2, true>(*st, tq, tk, tv, p, items, stream)
+                  : launch_attention<T, 2, false>(*st, tq, tk, tv, p, items, stream);
+  };
+  return dtype == 0 ? launch(__nv_bfloat16()) : launch(__half());
 }

@@ -87,6 +87,8 @@ template <class T>
 struct Pack16;
 template <>
 struct Pack16<__nv_bfloat16> {
+  using Two = __nv_bfloat162;
+  static __device__ __forceinline__ Two both(float a) { return __float2bfloat162_rn(a); }
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
@@ -97,6 +99,8 @@ struct Pack16<__nv_bfloat16> {
 };
 template <>
 struct Pack16<__half> {
+  using Two = __half2;
+  static __device__ __forceinline__ Two both(float a) { return __float2half2_rn(a); }
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
   }

@@ -368,3 +368,131 @@ def test_scores_that_are_not_finite(lk):
     assert torch.isnan(got[77, 1]).all()
     got[77, 1] = clean[77, 1]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lq,lk,D,group", [(300, 300, 128, 1), (130, 517, 64, 1), (3, 700, 128, 4), (260, 260, 72, 5), (1, 4000, 128, 2)])
+def test_values_that_causal_rows_do_not_see(lq, lk, D, group, dtype):
+    """A value row that is not finite reaches the rows that see its key, in its columns, and no other."""
+    q, k, v = qkv(lq, lk, 2 * group, 2, D, dtype, seed=13, spread=0.5)
+    clean = A.attention(q, k, v, causal=True)
+    keys = sorted({0, 5, lk // 2, max(lk - lq, 0), lk - lq // 2 - 1, lk - 2, lk - 1} & set(range(lk)))
+    for key in keys:
+        for bad in (math.nan, math.inf):
+            spoilt = v.clone()
+            spoilt[key, 1, 3] = bad
+            spoilt[key, 1, D - 1] = -bad
+            got = A.attention(q, k, spoilt, causal=True)
+            hit = torch.zeros(got.shape, dtype=torch.bool, device=DEV)
+            sees = torch.arange(lq, device=DEV) + lk - lq >= key
+            hit[:, group:, 3] = hit[:, group:, D - 1] = sees[:, None]
+            assert torch.equal(~torch.isfinite(got), hit), (key, bad)
+            assert torch.equal(got[~hit], clean[~hit])
+            if bad == math.inf:
+                assert (got[:, group:, 3][sees] == math.inf).all() and (got[:, group:, D - 1][sees] == -math.inf).all()
+
+
+def test_many_values_that_are_not_finite():
+    q, k, v = qkv(200, 200, 1, 1, 64, seed=14, spread=0.5)
+    clean = A.attention(q, k, v, causal=True)
+    v[90:] = math.nan
+    got = A.attention(q, k, v, causal=True)
+    assert torch.equal(got[:90], clean[:90]) and torch.isnan(got[90:]).all()
+
+
+def test_small_weights_of_a_long_row_count():
+    """One score far above 30000 others, whose weights together still matter: 16-bit weights must not lose them."""
+    for dtype in (torch.float16, torch.bfloat16):
+        n = 30000
+        q = torch.zeros(1, 1, 64, dtype=dtype, device=DEV)
+        q[0, 0, 0] = 8
+        k = torch.zeros(n, 1, 64, dtype=dtype, device=DEV)
+        k[777, 0, 0] = 14.0  # exp(14) = 1.2e6, the others 1 each
+        v = torch.ones(n, 1, 64, dtype=dtype, device=DEV)
+        v[777] = 0
+        check(q, k, v, [1], [n], cu=False)
+
+
+def test_strides_of_single_elements_do_not_matter():
+    q, k, v = qkv(1, 9, 4, 1, 64, seed=15)
+    want = A.attention(q, k, v)
+    odd = torch.as_strided(q, q.shape, (3, 64, 1))
+    assert torch.equal(A.attention(odd, torch.as_strided(k, k.shape, (64, 5, 1)), torch.as_strided(v, v.shape, (64, 1, 1))), want)
+    assert torch.equal(A.qk_norm_rope(odd), A.qk_norm_rope(q))
+
+
+# ------------------------------------------------------------------------------------------------ as they are used
+
+
+def test_joined_module_in_an_attention_block():
+    """Packed sequences through convrot projections, norms, rotation, attention and the out projection: the block's
+    module against the single calls, and those against the formulas on the projections' own outputs."""
+    from hyperflow_h3_flash_b200 import int8 as I
+    from hyperflow_h3_flash_b200 import synthetic, ulysses
+
+    T, width, heads, D = 410, 1024, 8, 128
+    layers = []
+    for i in range(4):
+        layer = I.Int8RotLinear(width, width, 256, bias=True)
+        synthetic.load_into(layer, synthetic.linear_weights(width, width, seed_offset=40 + i))
+        layers.append(layer.to(DEV))
+    core = A.QKNormAttention(D).to(DEV)
+    core.norm_q.weight.copy_(1 + _randn(D, seed=20, scale=0.2))
+    core.norm_k.weight.copy_(1 + _randn(D, seed=21, scale=0.2))
+    lens = [200, 0, 33, 177]
+    grid = torch.stack([torch.arange(T, device=DEV) // 60, torch.arange(T, device=DEV) // 10 % 6, torch.arange(T, device=DEV) % 10], 1)
+    table = A.rotary_table(grid, (44, 42, 42))
+    core.set_sequences(table, _cu(lens))
+    x = synthetic.activations(T, width, seed=22).to(DEV)
+    got = ulysses.attention_block_linears(x, *layers, heads, attention=core)
+    q, k, v = (layer(x).view(T, heads, D) for layer in layers[:3])
+    qn, kn = A.qk_norm_rope(q, k, q_weight=core.norm_q.weight, k_weight=core.norm_k.weight, table=table)
+    for g, t, w in ((qn, q, core.norm_q.weight), (kn, k, core.norm_k.weight)):
+        want, bound = norm_rope_reference(t, w, 1e-6, True, table, True)
+        assert ((g.double() - want).abs() <= bound).all()
+    o = check(qn, kn, v, lens, lens)
+    assert torch.equal(got, layers[3](o.reshape(T, width)))
+
+
+def test_captured_and_replayed():
+    from hyperflow_h3_flash_b200.graphs import CapturedCall
+
+    q, k, v = qkv(70, 2500, 4, 2, 128, seed=23)
+    table = A.rotary_table(torch.arange(70, device=DEV), (128,))
+
+    def call(q, k, v):
+        return A.attention(A.qk_norm_rope(q, table=table), k, v, causal=True)
+
+    assert _lib.lib().convrot_attention_workspace_size(70, 2500, 1, 4, 2, 128) > 0
+    first, second = CapturedCall(call, q, k, v), CapturedCall(call, q, k, v)  # two graphs, each with its own workspace
+    for seed in (24, 25, 26):
+        a, b = qkv(70, 2500, 4, 2, 128, seed=seed), qkv(70, 2500, 4, 2, 128, seed=seed + 10)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            two = second(*b)
+        one = first(*a)
+        torch.cuda.synchronize()
+        assert torch.equal(one, call(*a)) and torch.equal(two, call(*b))
+
+
+def test_calls_on_two_streams_at_once():
+    cases = [qkv(300, 3000, 4, 4, 64, seed=30 + i) for i in range(4)]
+    want = [A.attention(*c, causal=True) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(A.attention(*c, causal=True))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_more_items_than_the_grid_has_sms():
+    """Whole waves of items, and a last one that is divided among the SMs."""
+    q, k, v = qkv(4500, 2100, 12, 12, 64, seed=40)
+    check(q, k, v, [4500], [2100], cu=False)
+    lens = [1000, 1, 2048, 130, 1321]
+    check(q, torch.cat([k, k, k])[:4500], torch.cat([v, v, v])[:4500], lens, lens, True)
