@@ -1074,12 +1074,15 @@ __global__ void __launch_bounds__(kAtThreads, 1)
             tmem_st_32x32b_x16(s_addr + c * 16, pk);
           }
           if (again) break;
-          float mx[4] = {m, m, m, m};
+          float mx[2] = {m, m};
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-          const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+            for (int e = 0; e < 32; e += 4) {
+              mx[0] = max3(mx[0], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+              mx[1] = max3(mx[1], __uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]));
+            }
+          const float top = max3(mx[0], mx[1], mx[1]);
           // (rows without a query hold what was in shared memory: they must not ask for a rescaling at every tile)
           const bool grow = keys > 0 && (m == -CUDART_INF_F ? top != m : !((top - m) * c2 <= kRescaleLog2));
           if (!__any_sync(0xffffffffu, grow)) break;
