@@ -34,6 +34,20 @@ _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3
 MAX_HEAD_DIM = 128  # of attention; qk_norm_rope takes heads up to 256
 
 
+@functools.cache
+def _fast_calls():
+    """The compiled form of the common calls (csrc/fast_call.cpp), or None if it was not built: it calls the same C
+    entries, and answers None to every call that is not plainly in order, which then takes the way below."""
+    try:
+        from . import _fast
+    except ImportError:
+        return None
+    handle = _lib.lib()
+    names = ("rotary_table", "qk_norm_rope", "attention", "attention_workspace_size")
+    _fast.init(*(ctypes.cast(getattr(handle, f"convrot_{name}"), ctypes.c_void_p).value for name in names))
+    return _fast
+
+
 def _no_grad(*tensors: Tensor | None) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -91,6 +105,10 @@ def rotary_table(positions: Tensor, axes: Sequence[int], *, theta: float | Seque
     included; axis ``a`` turns ``axes[a] / 2`` pairs of channels, pair ``i`` by ``pos * theta[a] ** (-2 i / axes[a])``.
     Angles are formed and reduced in fp64, so far positions lose nothing.  Made once per clip and shared by every block:
     ``qk_norm_rope(table=...)`` reads it."""
+    if positions.is_cuda and (fast := _fast_calls()) is not None:
+        table = fast.rotary_table(positions, axes, theta)
+        if table is not None:
+            return table
     axes = tuple(int(d) for d in axes)
     if not 1 <= len(axes) <= 8 or any(d <= 0 or d % 2 for d in axes) or sum(axes) > 256:
         raise ValueError(f"axes must be 1 to 8 even positive widths of at most 256 channels in all, got {axes}")
@@ -163,6 +181,10 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
     (``rotary_table``'s, fp32 ``[T, R / 2, 2]``; None: no rotation): pairs of neighbours if ``interleaved``, else
     ``(j, j + R / 2)``.  fp32 arithmetic, one rounding.  Returns the new q (and k when given).  ``q_out`` / ``k_out`` may
     be the inputs themselves; an output that overlaps an input in any other way is not supported."""
+    if q_out is None and k_out is None and q.is_cuda and (fast := _fast_calls()) is not None:
+        made = fast.qk_norm_rope(q, k, q_weight, k_weight, eps, norm, table, interleaved)
+        if made is not None:
+            return made
     _no_grad(q, k, q_weight, k_weight)
     (T, Hq, D), qs = _heads(q, "q")
     if k is not None:
@@ -268,6 +290,10 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
 
     Scores, statistics and sums are fp32; the weights are rounded to the inputs' type for their product with v.  Few
     queries over long keys are split over the GPU and joined in a fixed order: results do not vary from run to run."""
+    if out is None and q.is_cuda and (fast := _fast_calls()) is not None:
+        made = fast.attention(q, k, v, cu_q, cu_k, causal, scale, return_lse)
+        if made is not None:
+            return made
     _no_grad(q, k, v)
     (Tq, Hq, D), qs = _heads(q, "q")
     (Tk, Hkv, Dk), ks = _heads(k, "k", q)

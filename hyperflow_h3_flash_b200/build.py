@@ -15,6 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libconvrot.so")
 SOURCES = sorted(os.path.join(HERE, "csrc", name) for name in os.listdir(os.path.join(HERE, "csrc"))
                  if name.endswith((".cu", ".cuh", ".h")))
+FAST = os.path.join(HERE, "_fast.so")
+FAST_SOURCE = os.path.join(HERE, "csrc", "fast_call.cpp")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "convrot.h")
 
 NVCC_FLAGS = [
@@ -31,15 +33,41 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found: set NVCC or put the CUDA toolkit on PATH")
 
 
-def stale() -> bool:
-    if not os.path.exists(LIB):
+def stale(built: str = LIB, sources: list[str] | None = None) -> bool:
+    if not os.path.exists(built):
         return True
-    built = os.path.getmtime(LIB)
-    return any(os.path.getmtime(src) > built for src in SOURCES + [HEADER])
+    when = os.path.getmtime(built)
+    return any(os.path.getmtime(src) > when for src in (SOURCES if sources is None else sources) + [HEADER])
+
+
+def build_fast(force: bool = False, verbose: bool = False) -> str:
+    """Compiles the Python module of the common calls (it links against torch and takes the library's entries at run
+    time); returns its path."""
+    if not force and not stale(FAST, [FAST_SOURCE]):
+        return FAST
+    import sysconfig
+
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    include = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], cuda]
+    tmp = FAST + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{d}" for d in include), "-o", tmp,
+           FAST_SOURCE, f"-L{os.path.join(base, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, FAST)
+    return FAST
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles the library if it is missing or older than its sources; returns its path."""
+    """Compiles the library, and the Python module beside it, if missing or older than their sources; returns the
+    library's path."""
+    build_fast(force, verbose)
     if not force and not stale():
         return LIB
     tmp = LIB + ".tmp"
