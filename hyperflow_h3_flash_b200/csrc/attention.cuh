@@ -594,6 +594,9 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(*tmem_holder);
+  grid_wait();  // what is above may run beside the end of the kernel before; nothing below may
+  // (not before the kernel that joins the parts: its blocks would gather on the first SMs that are free)
+  if (p.shares == 0) grid_release();
   const AttnGuard guard{smem_u32(const_cast<int*>(abort_flag)), p};
 
   // The next item, in every reading warp; false at the end of the work (or after a failed wait).  The warp is done with
@@ -1289,6 +1292,8 @@ __global__ void __launch_bounds__(kAtThreads, 1)
 // partial rows were just written and mostly come from L2.
 template <class T>
 __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_constant__ AttnParams p) {
+  grid_wait();
+  grid_release();
   const int lane = threadIdx.x & 31;
   const int shares = p.meta[0], items = p.meta[1], whole = p.meta[2], x = blockIdx.x;
   // (the limits also hold if the first kernel gave up and left no plan)

@@ -1,6 +1,24 @@
 // Host side of the attention operators (argument checks, tensor maps, launch shapes); included by convrot.cu inside its
 // unnamed namespace, after the device state and tensor-map helpers.  Contracts: include/convrot.h.
 
+// Launches a kernel that calls grid_wait() before it touches memory: its start overlaps the end of the one before.
+template <class... Params, class... Args>
+int launch_overlapped(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                      const Args&... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  return e == cudaSuccess ? CONVROT_OK : cuda_fail(e);
+}
+
 // ------------------------------------------------------------------------------------------------ rotary table
 
 int rotary_table(const void* pos, int pos_type, int64_t ld_pos, int64_t rows, int axes, const int* dims,
@@ -32,13 +50,11 @@ int rotary_table(const void* pos, int pos_type, int64_t ld_pos, int64_t rows, in
   const int64_t need = (rows * p.pairs + 255) / 256, most = 16 * static_cast<int64_t>(st->sms);
   const unsigned grid = static_cast<unsigned>(need < most ? need : most);
   switch (pos_type) {
-    case 0: rotary_table_kernel<int32_t><<<grid, 256, 0, stream>>>(p); break;
-    case 1: rotary_table_kernel<int64_t><<<grid, 256, 0, stream>>>(p); break;
-    case 2: rotary_table_kernel<float><<<grid, 256, 0, stream>>>(p); break;
-    default: rotary_table_kernel<double><<<grid, 256, 0, stream>>>(p); break;
+    case 0: return launch_overlapped(rotary_table_kernel<int32_t>, dim3(grid), 256, 0, stream, p);
+    case 1: return launch_overlapped(rotary_table_kernel<int64_t>, dim3(grid), 256, 0, stream, p);
+    case 2: return launch_overlapped(rotary_table_kernel<float>, dim3(grid), 256, 0, stream, p);
+    default: return launch_overlapped(rotary_table_kernel<double>, dim3(grid), 256, 0, stream, p);
   }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? CONVROT_OK : cuda_fail(e);
 }
 
 // ------------------------------------------------------------------------------------------------ norm and rotation
@@ -101,21 +117,9 @@ int qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t q
   p.inv_D = 1.0f / static_cast<float>(D);
   const int64_t blocks = (rows * p.items + kRopeWarps - 1) / kRopeWarps;
   if (blocks > INT32_MAX) return CONVROT_ERR_SHAPE;
-  const unsigned grid = static_cast<unsigned>(blocks);
-  const int threads = kRopeWarps * 32;
-  if (dtype == 0) {
-    if (single)
-      qk_norm_rope_kernel<__nv_bfloat16, true><<<grid, threads, 0, stream>>>(p);
-    else
-      qk_norm_rope_kernel<__nv_bfloat16, false><<<grid, threads, 0, stream>>>(p);
-  } else {
-    if (single)
-      qk_norm_rope_kernel<__half, true><<<grid, threads, 0, stream>>>(p);
-    else
-      qk_norm_rope_kernel<__half, false><<<grid, threads, 0, stream>>>(p);
-  }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? CONVROT_OK : cuda_fail(e);
+  auto kernel = dtype == 0 ? (single ? qk_norm_rope_kernel<__nv_bfloat16, true> : qk_norm_rope_kernel<__nv_bfloat16, false>)
+                           : (single ? qk_norm_rope_kernel<__half, true> : qk_norm_rope_kernel<__half, false>);
+  return launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), kRopeWarps * 32, 0, stream, p);
 }
 
 // ------------------------------------------------------------------------------------------------ attention
@@ -179,15 +183,12 @@ int launch_attention(const DeviceState& st, const CUtensorMap& tq, const CUtenso
     if (e != cudaSuccess) return cuda_fail(e);
     store_resident(reinterpret_cast<const void*>(kernel), 1);
   }
-  kernel<<<static_cast<unsigned>(items), kAtThreads, AttnCfg<NP>::kSmemBytes, stream>>>(tq, tk, tv, p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e);
-  if (p.shares > 0) {
-    // a warp for each row that an item has at most (few tokens have few)
-    const int positions = p.Tq < 2 * p.positions ? p.Tq : 2 * p.positions;
-    attention_combine_kernel<T><<<dim3(p.shares, (positions * p.group + 7) / 8), 256, 0, stream>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e);
-  }
-  return CONVROT_OK;
+  rc = launch_overlapped(kernel, dim3(static_cast<unsigned>(items)), kAtThreads, AttnCfg<NP>::kSmemBytes, stream, tq, tk,
+                         tv, p);
+  if (rc || p.shares == 0) return rc;
+  // a warp for each row that an item has at most (few tokens have few)
+  const int positions = p.Tq < 2 * p.positions ? p.Tq : 2 * p.positions;
+  return launch_overlapped(attention_combine_kernel<T>, dim3(p.shares, (positions * p.group + 7) / 8), 256, 0, stream, p);
 }
 
 int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v,

@@ -23,6 +23,12 @@
 
 namespace convrot {
 
+// A kernel launched with programmatic stream serialisation may begin while the one before it in the stream ends:
+// grid_wait() holds until that one is complete and its writes are visible, and has to come before the first access to
+// memory; grid_release() lets the next such kernel begin as soon as this one's last blocks are placed.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 constexpr int kRopeMaxPairs = 128;
 constexpr int kRopeMaxAxes = 8;
 
@@ -47,6 +53,8 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant
     axis[threadIdx.x] = p.axis[threadIdx.x];
   }
   __syncthreads();
+  grid_wait();
+  grid_release();
   const int64_t n = p.rows * p.pairs;
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += step) {
@@ -152,6 +160,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __g
   constexpr int CH = INTERLEAVED ? 1 : 2;  // 8-channel pieces of a lane
   constexpr int kSteps = kRopeRows / CH;
   constexpr int kPartner = INTERLEAVED ? 1 : 8;
+  grid_wait();
+  grid_release();
   const int lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kRopeWarps + (threadIdx.x >> 5);
   if (item >= p.rows * p.items) return;  // whole warps
