@@ -288,7 +288,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
     * A query that sees no key gives zeros (and ``-inf`` in the log-sum-exp).
     * ``return_lse`` adds the natural log-sum-exp of each row's scores, fp32 ``[Tq, Hq]``.
 
-    Scores, statistics and sums are fp32; the weights are rounded to the inputs' type for their product with v.  Few
+    ``out`` must not overlap the inputs.  Scores, statistics and sums are fp32; the weights are rounded to the inputs' type for their product with v.  Few
     queries over long keys are split over the GPU and joined in a fixed order: results do not vary from run to run."""
     if out is None and q.is_cuda and (fast := _fast_calls()) is not None:
         made = fast.attention(q, k, v, cu_q, cu_k, causal, scale, return_lse)

@@ -496,3 +496,69 @@ def test_more_items_than_the_grid_has_sms():
     check(q, k, v, [4500], [2100], cu=False)
     lens = [1000, 1, 2048, 130, 1321]
     check(q, torch.cat([k, k, k])[:4500], torch.cat([v, v, v])[:4500], lens, lens, True)
+
+
+def test_offsets_beyond_32_bits():
+    """Queries, keys, values and outputs as columns of one wide buffer whose rows reach past 2^31 elements."""
+    T, width = 34000, 65536
+    buf = torch.empty(T, width, dtype=torch.bfloat16, device=DEV)
+    parts = [buf[:, i * 128 : (i + 1) * 128].unflatten(1, (1, 128)) for i in range(4)]
+    for i, t in enumerate(parts[:3]):
+        t.copy_(_randn(T, 1, 128, seed=50 + i, dtype=torch.bfloat16))
+    q, k, v, out = parts
+    dense = [t.contiguous() for t in (q, k, v)]
+    for causal in (False, True):
+        A.attention(q, k, v, causal=causal, out=out)
+        assert torch.equal(out, A.attention(*dense, causal=causal))
+    few = A.attention(q[-3:], k, v, causal=True)  # single tokens: the keys are divided
+    assert torch.equal(few, A.attention(dense[0][-3:], *dense[1:], causal=True))
+    table = A.rotary_table(torch.arange(T, device=DEV), (128,))
+    A.qk_norm_rope(q, k, table=table, q_out=out, k_out=k)
+    assert torch.equal(out, A.qk_norm_rope(dense[0], table=table)) and torch.equal(k, A.qk_norm_rope(dense[1], table=table))
+    A.qk_norm_rope(q, table=table, interleaved=False, q_out=q)
+    assert torch.equal(q, A.qk_norm_rope(dense[0], table=table, interleaved=False))
+
+
+def test_compiled_and_interpreted_calls_agree():
+    """The compiled form of a call gives what the checked one gives, and hands over what it does not take."""
+    fast = A._fast_calls()
+    assert fast is not None
+    q, k, v = qkv(40, 40, 4, 2, 64, seed=60)
+    table = A.rotary_table(torch.arange(40, device=DEV), (64,))
+    w = torch.ones(64, device=DEV)
+    quick = fast.qk_norm_rope(q, k, w, None, 1e-6, True, table, True)
+    slow = A.qk_norm_rope(q, k, q_weight=w, table=table, q_out=torch.empty_like(q), k_out=torch.empty_like(k))
+    assert all(torch.equal(a, b) for a, b in zip(quick, slow))
+    quick, lse = fast.attention(q, k, v, None, None, True, None, True)
+    slow, slow_lse = A.attention(q, k, v, causal=True, out=torch.empty_like(q), return_lse=True)
+    assert torch.equal(quick, slow) and torch.equal(lse, slow_lse)
+    cu = _cu([40])
+    for args in ((q.cpu(), k, v, None, None, True, None, False), (q, k.half(), v, None, None, True, None, False),
+                 (q, k, v[:3], None, None, True, None, False), (q, k, v, cu, None, True, None, False),
+                 (q, k, v, cu.long(), cu, True, None, False), (q, k, v, None, None, True, -1.0, False),
+                 (q.clone().requires_grad_(), k, v, None, None, True, None, False),
+                 (q, k[:, :0], v[:, :0], None, None, True, None, False), (q, k, v, None, None, 1, None, False),
+                 (q, k, v, None, None, True, "x", False), (q, k, v)):
+        assert fast.attention(*args) is None
+    for args in ((q, k[:5], None, None, 1e-6, True, table, True), (q, k, w[:3], None, 1e-6, True, table, True),
+                 (q, k, w, w.bfloat16(), 1e-6, True, table, True), (q, None, None, w, 1e-6, True, table, True),
+                 (q, k, w, None, 1e-6, False, table, True), (q, k, None, None, math.nan, True, table, True),
+                 (q, k, None, None, 1e-6, False, None, True), (q, k, None, None, 1e-6, True, table.double(), True),
+                 (q, k, None, None, 1e-6, True, table[:, :3], True)):
+        assert fast.qk_norm_rope(*args) is None
+    for args in ((table, (64,), 1e4), (torch.arange(4, device=DEV)[:, None], (63,), 1e4),
+                 (torch.arange(4, device=DEV)[:, None], (64,), 0.0), (torch.arange(4, device=DEV)[:, None], (64, 64), 1e4)):
+        assert fast.rotary_table(*args) is None
+
+
+def test_refusals_on_the_gpu_leave_the_device_usable():
+    q, k, v = qkv(8, 8, 2, 2, 64, seed=61)
+    wide = torch.empty(8, 2, 65, dtype=torch.bfloat16, device=DEV)
+    for bad in (lambda: A.attention(q.float(), k.float(), v.float()), lambda: A.attention(wide[..., 1:], k, v),
+                lambda: A.attention(q, k.expand(8, 2, 64)[:, :1].expand(8, 2, 64), v), lambda: A.qk_norm_rope(q.float()),
+                lambda: A.qk_norm_rope(wide[..., 1:]), lambda: A.qk_norm_rope(q, k, q_out=k),
+                lambda: A.attention(q, k, v, cu_q=torch.zeros(2, dtype=torch.int32), cu_k=torch.zeros(2, dtype=torch.int32)),
+                lambda: A.rotary_table(torch.zeros(3, 2, dtype=torch.int16, device=DEV), (8, 8))):
+        with pytest.raises(ValueError):
+            bad()
+    check(q, k, v, [8], [8], cu=False)
