@@ -498,28 +498,6 @@ __device__ __forceinline__ int launch_cancelled(uint32_t answer) {
   return got ? x : -1;
 }
 
-// Two fp32 lanes in a 64-bit register (one issue slot for both).
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // Weights 2^(c2 s + neg) of 32 scores, their sums (two lanes of two), and the weights in 16 bits.  All of them on the
 // special-function unit: one in 2, 3, 4, 8 or 16 of them by a quartic on the FMA pipe shortened this step, but the
 // kernel took 3 to 13 % longer at 128 channels (more issue slots beside the MMA warp, and a lower clock under the power

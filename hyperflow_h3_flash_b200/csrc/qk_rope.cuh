@@ -9,11 +9,12 @@
 //
 // qk_norm_rope_kernel: for each head row x of q and k
 //   y = x * rsqrt(mean(x^2) + eps) * w,   (a, b) -> (a c - b s, b c + a s) for each pair of the first R channels,
-// all in fp32, rounded once to the output type.  Bound by HBM (each row read once, written once; 8 fp32 operations per
-// element).  A lane holds 8 neighbouring channels (one 16-byte load), a row lies in a power-of-two group of lanes, so
-// the sum of squares is a few shuffles and the statistics never touch memory; pairs half a rotated width apart reach
-// each other by shuffles as well.  A warp takes kRopeRows row groups of one token at once: that many independent loads
-// in flight per lane, and one read of the token's table row for all of them.
+// all in fp32, rounded once to the output type.  Bound by HBM (each row read once, written once): 32760 tokens of 2 x 40
+// heads of 128 take 221 us, 6.1 TB/s (231 with pairs half the rotated width apart; a plain copy of the same bytes 205),
+// ncu sees the issue slots as the next bound.  A lane holds 8 neighbouring channels (one 16-byte load) or two such
+// pieces, so that both channels of a pair are always its own; a row lies in a power-of-two group of lanes, so the sum of
+// squares is a few shuffles and the statistics never touch memory.  A warp takes several rows of one token at once:
+// kRopeRows independent loads in flight per lane, and one read of the token's table row for all of them.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -28,6 +29,33 @@ namespace convrot {
 // memory; grid_release() lets the next such kernel begin as soon as this one's last blocks are placed.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Two fp32 lanes in a 64-bit register (one issue slot for both).
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 constexpr int kRopeMaxPairs = 128;
 constexpr int kRopeMaxAxes = 8;
@@ -139,27 +167,18 @@ __device__ __forceinline__ void load_weight8(const void* w, int f32, int c, floa
   }
 }
 
-template <class T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
-  const uint32_t v[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = Pack16<T>::unpack(v[i]);
-    x[2 * i] = f.x, x[2 * i + 1] = f.y;
-  }
-}
-
 // A warp item is a few steps of rows of q or of k of one token.  Weights and rotation are joined once for all of an item's
 // rows: with (a, b) a pair and a' = inv a, b' = inv b, out = (a' (wa c) - b' (wb s), b' (wb c) + a' (wa s)), so a row
-// costs two operations an element beside its sum of squares and the scale.  (Every row with its own weight and rotation
-// took 350 us for 32760 tokens x 2 x 40 heads of 128, bound by issue slots.)  With pairs of neighbours a lane holds 8
-// channels; with pairs R / 2 apart it holds the 8 channels and their partners, R / 2 further (by shuffles from the
-// partners' lane they cost 306 us instead of 239), and lanes behind the rotated part hold 16 channels in a row.
+// costs two operations an element beside its sum of squares and the scale, and two channels go through each as one
+// paired instruction.  (For 32760 tokens x 2 x 40 heads of 128: every row with its own weight and rotation 350 us, bound
+// by issue slots; unpaired 223, and 238 with pairs R / 2 apart.)  With pairs of neighbours a lane holds 8 channels; with
+// pairs R / 2 apart it holds the 8 channels and their partners, R / 2 further (fetched by shuffles from the partners'
+// lane they cost 306 us), and lanes behind the rotated part hold 16 channels in a row.
 template <class T, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __grid_constant__ QkRopeParams p) {
   constexpr int CH = INTERLEAVED ? 1 : 2;  // 8-channel pieces of a lane
   constexpr int kSteps = kRopeRows / CH;
-  constexpr int kPartner = INTERLEAVED ? 1 : 8;
+  constexpr int kPartner = INTERLEAVED ? 1 : 4;  // registers of two channels
   grid_wait();
   grid_release();
   const int lane = threadIdx.x & 31;
@@ -197,70 +216,89 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __g
         raw[r][h] = __ldcs(reinterpret_cast<const uint4*>(in + r * per * in_h + h * apart));
     }
 
-  // out[i] = mine[i] x[i] + other[i] x[i's partner]
-  float mine[8 * CH], other[8 * CH];
+  // Two channels to a register, so that an instruction works on both: with pairs of neighbours channels (0, 2), (1, 3),
+  // (4, 6), (5, 7), else neighbours; element i's partner is i ^ kPartner either way, with kPartner = 1 or 4 registers.
+  // out[i] = mine[i] x[i] + other[i] x[i ^ kPartner]
+  constexpr int kRegs = 4 * CH;
+  uint64_t mine[kRegs], other[kRegs];
+  {
+    float m[8 * CH], o[8 * CH];
 #pragma unroll
-  for (int h = 0; h < CH; ++h) {
-    float w[8] = {};
-    if (here[h]) load_weight8<T>(is_k ? p.weight[1] : p.weight[0], p.weight_f32, c + h * apart, w);
+    for (int h = 0; h < CH; ++h) {
+      float w[8] = {};
+      if (here[h]) load_weight8<T>(is_k ? p.weight[1] : p.weight[0], p.weight_f32, c + h * apart, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mine[8 * h + i] = w[i];
-  }
-  if (p.table && turns) {
-    const float4* src =
-        reinterpret_cast<const float4*>(p.table + t * p.ld_table + (INTERLEAVED ? c >> 1 : c));
+      for (int i = 0; i < 8; ++i) m[8 * h + i] = w[i], o[8 * h + i] = 0.0f;
+    }
+    if (p.table && turns) {
+      constexpr int kApart = INTERLEAVED ? 1 : 8;
+      const float4* src = reinterpret_cast<const float4*>(p.table + t * p.ld_table + (INTERLEAVED ? c >> 1 : c));
 #pragma unroll
-    for (int i = 0; i < 2 * CH; ++i) {
-      const float4 f = __ldg(src + i);
-      const float cs[2] = {f.x, f.z}, sn[2] = {f.y, f.w};
+      for (int i = 0; i < 2 * CH; ++i) {
+        const float4 f = __ldg(src + i);
+        const float cs[2] = {f.x, f.z}, sn[2] = {f.y, f.w};
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int a = INTERLEAVED ? 4 * i + 2 * k : 2 * i + k, b = a + kPartner;
-        const float wa = mine[a], wb = mine[b];
-        mine[a] = wa * cs[k], other[a] = -wb * sn[k];
-        mine[b] = wb * cs[k], other[b] = wa * sn[k];
+        for (int k = 0; k < 2; ++k) {
+          const int a = INTERLEAVED ? 4 * i + 2 * k : 2 * i + k, b = a + kApart;
+          const float wa = m[a], wb = m[b];
+          m[a] = wa * cs[k], o[a] = -wb * sn[k];
+          m[b] = wb * cs[k], o[b] = wa * sn[k];
+        }
       }
+    }
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) {
+      const int a = INTERLEAVED ? (i >> 1) * 4 + (i & 1) : 2 * i, b = INTERLEAVED ? a + 2 : a + 1;
+      mine[i] = pack2(m[a], m[b]);
+      other[i] = pack2(o[a], o[b]);
     }
   }
 
 #pragma unroll
   for (int r = 0; r < kSteps; ++r) {
-    float x[8 * CH], y[8 * CH];
+    uint64_t x[kRegs];
 #pragma unroll
     for (int h = 0; h < CH; ++h) {
       const uint32_t v[4] = {raw[r][h].x, raw[r][h].y, raw[r][h].z, raw[r][h].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = Pack16<T>::unpack(v[i]);
-        x[8 * h + 2 * i] = f.x, x[8 * h + 2 * i + 1] = f.y;
+      for (int i = 0; i < 4; i += 2) {
+        const float2 f = Pack16<T>::unpack(v[i]), g = Pack16<T>::unpack(v[i + 1]);
+        x[4 * h + i] = INTERLEAVED ? pack2(f.x, g.x) : pack2(f.x, f.y);
+        x[4 * h + i + 1] = INTERLEAVED ? pack2(f.y, g.y) : pack2(g.x, g.y);
       }
     }
     if (p.norm) {
-      float s0 = 0.0f, s1 = 0.0f;
+      uint64_t s2 = 0;
 #pragma unroll
-      for (int i = 0; i < 8 * CH; i += 2) s0 = fmaf(x[i], x[i], s0), s1 = fmaf(x[i + 1], x[i + 1], s1);
-      float sum = s0 + s1;
+      for (int i = 0; i < kRegs; ++i) s2 = fma2(x[i], x[i], s2);
+      const float2 s = unpack2(s2);
+      float sum = s.x + s.y;
       for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       const float inv = rsqrtf(fmaf(sum, p.inv_D, p.eps));
 #pragma unroll
-      for (int i = 0; i < 8 * CH; ++i) x[i] *= inv;
+      for (int i = 0; i < kRegs; ++i) x[i] = mul2(x[i], pack2(inv, inv));
     }
+    float2 y[kRegs];
     if (p.table && turns) {
 #pragma unroll
-      for (int i = 0; i < 8 * CH; ++i) y[i] = fmaf(x[i], mine[i], x[i ^ kPartner] * other[i]);
+      for (int i = 0; i < kRegs; ++i) y[i] = unpack2(fma2(x[i], mine[i], mul2(x[i ^ kPartner], other[i])));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8 * CH; ++i) y[i] = x[i] * mine[i];
+      for (int i = 0; i < kRegs; ++i) y[i] = unpack2(mul2(x[i], mine[i]));
     }
 #pragma unroll
     for (int h = 0; h < CH; ++h)
       if (here[h] && row0 + r * per < heads) {
-        uint4 u;
-        u.x = Pack16<T>::pack(y[8 * h], y[8 * h + 1]);
-        u.y = Pack16<T>::pack(y[8 * h + 2], y[8 * h + 3]);
-        u.z = Pack16<T>::pack(y[8 * h + 4], y[8 * h + 5]);
-        u.w = Pack16<T>::pack(y[8 * h + 6], y[8 * h + 7]);
-        __stcs(reinterpret_cast<uint4*>(out + r * per * out_h + h * apart), u);
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = 4 * h + i;
+          if (INTERLEAVED)
+            u[i] = (i & 1) ? Pack16<T>::pack(y[k - 1].y, y[k].y) : Pack16<T>::pack(y[k].x, y[k + 1].x);
+          else
+            u[i] = Pack16<T>::pack(y[k].x, y[k].y);
+        }
+        __stcs(reinterpret_cast<uint4*>(out + r * per * out_h + h * apart), make_uint4(u[0], u[1], u[2], u[3]));
       }
   }
 }
