@@ -268,7 +268,13 @@ def _attention_torch(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor | None, cu_k:
             s = s.masked_fill(~seen, -math.inf)
         z = torch.logsumexp(s, dim=-1) if k1 > k0 else s.new_full(s.shape[:2], -math.inf)
         w = torch.exp(s - torch.where(z == -math.inf, 0.0, z)[..., None])
-        out[q0:q1] = (w @ vf).transpose(0, 1).to(q.dtype)
+        o = w @ vf
+        if causal and not vf.isfinite().all():  # a weight of zero does not keep a NaN or an infinity out of a product
+            o = w @ vf.nan_to_num(0.0, 0.0, 0.0)
+            for key in (~vf.isfinite()).any(2).any(0).nonzero().flatten().tolist():
+                value = torch.where(vf[:, key].isfinite(), 0.0, vf[:, key])
+                o += torch.where(seen[:, key, None], value[:, None], 0.0)
+        out[q0:q1] = o.transpose(0, 1).to(q.dtype)
         if lse is not None:
             lse[q0:q1] = z.transpose(0, 1)
 
@@ -288,8 +294,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
     * A query that sees no key gives zeros (and ``-inf`` in the log-sum-exp).
     * ``return_lse`` adds the natural log-sum-exp of each row's scores, fp32 ``[Tq, Hq]``.
 
-    ``out`` must not overlap the inputs.  Scores, statistics and sums are fp32; the weights are rounded to the inputs' type for their product with v.  Few
-    queries over long keys are split over the GPU and joined in a fixed order: results do not vary from run to run."""
+    ``out`` must not overlap the inputs, nor its rows each other.  Scores, statistics and sums are fp32; the weights are
+    rounded to the inputs' type for their product with v.  Few queries over long keys are split over the GPU and joined
+    in a fixed order: results do not vary from run to run."""
     if out is None and q.is_cuda and (fast := _fast_calls()) is not None:
         made = fast.attention(q, k, v, cu_q, cu_k, causal, scale, return_lse)
         if made is not None:
@@ -319,6 +326,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
             raise ValueError(f"cu_q and cu_k must have one length, got {cu_q.shape[0]} and {cu_k.shape[0]}")
         batch = cu_q.shape[0] - 1
     out = _output(out, q, "out")
+    if Tq and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+        raise ValueError("out must not be one of the inputs")
     lse = torch.empty(Tq, Hq, dtype=torch.float32, device=q.device) if return_lse else None
     if not q.is_cuda:
         _attention_torch(q, k, v, cu_q, cu_k, causal, scale, out, lse)

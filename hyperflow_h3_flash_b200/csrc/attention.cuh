@@ -20,13 +20,14 @@
 // p is rounded to the inputs' 16-bit type (a tcgen05 product takes both operands in one type; half a step relative per
 // weight, the same as the output's own rounding); l sums the unrounded p.
 //
-// What bounds it.  A step of two 128 x 128 tiles at 128 channels needs 2048 cycles of the tensor pipe and as many of the
-// special-function unit (2^15 exponentials at 16 a cycle); it takes about 3100, since the weights of a tile depend on its
-// scores and the next scores go where the weights were: the two tiles cover each other's latency only in part.  ncu on
-// 8192 tokens x 18 heads: tensor pipe 67 % of active cycles, special-function unit 67 %.  32760 tokens x 5 heads: 1.93
-// ms, 1420 TFLOP/s (causal 1.01 ms, 1360) in a burst; 1220 over seconds, where the 1000 W limit brings the clock to 1.5
-// GHz.  Single tokens over long caches: 5.3 TB/s of keys and values.  Short keys (333) pay 6000 to 8000 cycles an item for
-// its first tile, its output and the cold code of both, beside 9500 of steps: 272 us for 32760 x 40 heads.
+// What bounds it.  A step of two 128 x 128 tiles at 128 channels needs 2048 cycles of the tensor pipe and as many of
+// the special-function unit (2^15 exponentials at 16 a cycle); it takes about 3100, since the weights of a tile depend
+// on its scores and the next scores go where the weights were: the two tiles cover each other's latency only in part.
+// ncu on 8192 tokens x 18 heads: tensor pipe 67 % of active cycles, special-function unit 67 %.  32760 tokens x 5
+// heads: 1.94 ms, 1415 TFLOP/s (causal 1.03 ms, 1330) in a burst; 1220 over seconds, where the 1000 W limit brings the
+// clock to 1.5 GHz.  Single tokens over long caches: 5.3 TB/s of keys and values.  Short keys (333) pay 6000 to 8000
+// cycles an item for its first tile, its output and the cold code of both, beside 9500 of steps: 272 us for 32760 x 40
+// heads.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -47,7 +48,7 @@ constexpr int kAtThreads = 384;
 constexpr int kAtPanelBytes = 128 * 128;  // 128 rows x 64 channels of 16 bits, 128-byte swizzled rows
 constexpr uint64_t kDrainNs = 1000000000ull;  // for work of its own that a CTA that gave up has still in flight
 constexpr float kRescaleLog2 = 8.0f;
-constexpr int kFirstSteps = 6;  // 16-key steps of a tile's weights that are handed over before the rest
+constexpr int kFirstSteps = 6;  // 16-key steps of a tile's weights (three of four pieces) handed over before the rest
 
 constexpr int kItems = 4;        // items on their way through the CTA
 constexpr int kBadWords = 13;     // of an item: any, and a bit for each key of the (at most 3) tiles seen in part
@@ -59,7 +60,8 @@ struct AttnCfg {  // NP: 64-channel panels of a head (1: D <= 64, 2: D <= 128)
   static constexpr int kStages = NP == 2 ? 4 : 8;
   static constexpr int kStageOut = 4096;  // output staging of a warp: 32 rows of 128 bytes
   static constexpr int kNumBars = 2 * kStages + 19 + 3 * kItems;
-  static constexpr int kSmallBytes = 8 * kNumBars + kItems * 48 + 2 * 16 + 5 * kMaxShares + 4 + 16 + 4 * kItems * kBadWords;
+  static constexpr int kSmallBytes =
+      8 * kNumBars + kItems * 48 + 2 * 16 + 5 * kMaxShares + 4 + 16 + 4 * kItems * kBadWords;
   static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 8 * kStageOut + kSmallBytes + 1024;
   static constexpr int kO = 256;  // TMEM columns from S_i to O_i
 };
@@ -97,9 +99,9 @@ struct AttnParams {
 // balance without a counter in memory, no start-up between items, and the loads of the next item begin while the last
 // tiles of this one are multiplied.  Causal items come longest first within a head.
 //
-// Where the last wave of items would leave SMs idle, its items are divided evenly (AttnParams::shares): share s of G gets
-// the s-th G-th of their key tiles, whichever items these lie in.  32760 tokens x 5 heads are 640 items on 148 SMs, 5
-// waves for 4.3 waves of work.
+// Where the last wave of items would leave SMs idle, its items are divided evenly (AttnParams::shares): share s of G
+// gets the s-th G-th of their key tiles, whichever items these lie in.  32760 tokens x 5 heads are 640 items on 148
+// SMs, 5 waves for 4.3 waves of work.
 //
 // An item of a single query tile (a sequence's last one, or a few new tokens over a long cache) uses both softmax
 // groups all the same: tile 0 takes the even key tiles and tile 1 the odd ones, each with its own m, l and o, joined at
@@ -211,7 +213,8 @@ struct AttnWalk {
       a.k0 = __shfl_sync(0xffffffffu, k0, src);
       a.lk = __shfl_sync(0xffffffffu, lk, src);
       attn_place(p, rel - __shfl_sync(0xffffffffu, upto - mine, src), a);
-      return true;
+      // (the items of sequences that overlap, which the arrays must not hold, can pass 32 bits)
+      return a.pos >= 0 && a.pos < a.lq && a.head >= 0 && a.head < p.heads_kv;
     }
     return false;
   }
@@ -564,7 +567,8 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   if (threadIdx.x == 0) {
     for (int b = 0; b < Cfg::kNumBars; ++b) {
       const int c = b - 2 * S;
-      mbar_init(&bars[b], (c >= 8 && c < 12) || c == 15 || c == 16 ? 4 : c >= 19 + kItems && c < 19 + 2 * kItems ? kReaders : 1);
+      const bool by_warps = (c >= 8 && c < 12) || c == 15 || c == 16, by_readers = c >= 19 + kItems && c < 19 + 2 * kItems;
+      mbar_init(&bars[b], by_warps ? 4 : by_readers ? kReaders : 1);
     }
     *abort_flag = 0;
     fence_mbarrier_init();
@@ -614,9 +618,8 @@ __global__ void __launch_bounds__(kAtThreads, 1)
     setmaxnreg_dec<56>();
     if (warp == 11) {
       // -------------------------------------------------------------- scheduler
-      // (One call site for each piece of work: the instruction cache is shared with the loops that matter.  Unrolled and
-      // called from several places this warp's code was 66 of the kernel's 157 KB, and every cold path ran at 10 to 15
-      // cycles an instruction.)
+      // (One call site for each piece of work: unrolled and called from several places this warp's code was 66 of the
+      // kernel's 157 KB.)
       AttnWalk walk;
       AttnPlace a;
       const int items = attn_count(p, lane);
@@ -650,7 +653,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
               for (int i = lane; i <= sh.items; i += 32) p.meta[4 + i] = sh.items ? pre[i] : 0;
               if (lane == 0) p.meta[0] = sh.shares, p.meta[1] = sh.items, p.meta[2] = whole;
             }
-            if (s < sh.shares) {
+            if (sh.total > 0 && s < sh.shares) {  // (without items, pre and units hold nothing)
 #pragma unroll 1
               for (int k = 0; k < 2; ++k) {
                 x = end;
@@ -905,8 +908,8 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       // -------------------------------------------------------------- values that a row of the tile must not meet
       // A weight of zero does not keep a NaN or an infinity out of a product.  Rows behind a sequence's end (another
       // request's) are cleared.  In the tiles that causal rows see in part, values that are not finite are cleared and
-      // their keys noted: the rows that do see them get those values with the output.  (Rows behind the tensor's end are zeros
-      // that TMA filled in.)
+      // their keys noted: the rows that do see them get those values with the output.  (Rows behind the tensor's end
+      // are zeros that TMA filled in.)
       uint32_t slot = 0, fixes = 0;
       while (next_item()) {
         uint32_t* noted = bad + (item_count % kItems) * kBadWords;
@@ -934,7 +937,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
 #pragma unroll 1
             for (int c = 0; c < NP; ++c) {
 #pragma unroll 8
-              for (int r = 0; r < kAtTile; r += 4) {  // 8 lanes for each of 4 rows (rows behind the end are zeros by now)
+              for (int r = 0; r < kAtTile; r += 4) {  // 8 lanes for each of 4 rows (zeros behind the end by now)
                 const uint4 v = *reinterpret_cast<const uint4*>(tile + c * kAtPanelBytes + r * 128 + lane * 16);
                 sum[0] = __hfma2(*reinterpret_cast<const T2*>(&v.x), zero, sum[0]);
                 sum[1] = __hfma2(*reinterpret_cast<const T2*>(&v.y), zero, sum[1]);
@@ -1094,13 +1097,12 @@ __global__ void __launch_bounds__(kAtThreads, 1)
             }
           }
         }
-        if (kFirstSteps == 4) hand_over(0);
 #pragma unroll
         for (int c = 2; c < 4; ++c) {
           uint32_t pk[16];
           weights<T>(s[c], c2, neg, sum, pk);
           tmem_st_32x32b_x16(s_addr + c * 16, pk);
-          if (c == 2 && kFirstSteps == 6) hand_over(0);
+          if (c == 2) hand_over(0);
         }
         hand_over(1);
         const float2 a = unpack2(add2(sum[0], sum[1]));
@@ -1277,9 +1279,9 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   }
 }
 
-// Joins the parts of the items that were divided: o = sum_s w_s o_s with w_s = 2^(lse_s - m) / sum 2^(lse_s - m), in the
-// order of the shares.  Block (x, y): rows y, y + gridDim.y, ... (by eights) of the x-th divided item; one warp a row.  The
-// partial rows were just written and mostly come from L2.
+// Joins the parts of the items that were divided: o = sum_s w_s o_s with w_s = 2^(lse_s - m) / sum 2^(lse_s - m), in
+// the order of the shares.  Block (x, y): rows y, y + gridDim.y, ... (by eights) of the x-th divided item; one warp a
+// row.  The partial rows were just written and mostly come from L2.
 template <class T>
 __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_constant__ AttnParams p) {
   grid_wait();

@@ -59,6 +59,13 @@ int rotary_table(const void* pos, int pos_type, int64_t ld_pos, int64_t rows, in
 
 // ------------------------------------------------------------------------------------------------ norm and rotation
 
+// Whether rows of D elements, a x b of them, may share an element (the stride of a single one does not count).
+bool rows_overlap(int64_t a, int64_t stride_a, int64_t b, int64_t stride_b, int D) {
+  if (a <= 1) return b > 1 && stride_b < D;
+  if (b <= 1) return stride_a < D;
+  return stride_a < stride_b ? stride_a < D || stride_b / a < stride_a : stride_b < D || stride_a / b < stride_b;
+}
+
 int qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h, int heads_q,
                  const void* k, int64_t k_t, int64_t k_h, void* k_out, int64_t ko_t, int64_t ko_h, int heads_k,
                  int64_t rows, int D, int dtype, int norm, const void* q_weight, const void* k_weight, int weight_f32,
@@ -85,6 +92,8 @@ int qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t q
     if (strides[i] < 0) return CONVROT_ERR_SHAPE;
     if (strides[i] % 8) return CONVROT_ERR_ALIGN;
   }
+  if (rows_overlap(rows, qo_t, heads_q, qo_h, D) || (heads_k && rows_overlap(rows, ko_t, heads_k, ko_h, D)))
+    return CONVROT_ERR_SHAPE;
   if (!aligned16(q) || !aligned16(q_out) || !aligned16(k) || !aligned16(k_out) || !aligned16(q_weight) ||
       !aligned16(k_weight))
     return CONVROT_ERR_ALIGN;
@@ -117,8 +126,9 @@ int qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t q
   p.inv_D = 1.0f / static_cast<float>(D);
   const int64_t blocks = (rows * p.items + kRopeWarps - 1) / kRopeWarps;
   if (blocks > INT32_MAX) return CONVROT_ERR_SHAPE;
-  auto kernel = dtype == 0 ? (single ? qk_norm_rope_kernel<__nv_bfloat16, true> : qk_norm_rope_kernel<__nv_bfloat16, false>)
-                           : (single ? qk_norm_rope_kernel<__half, true> : qk_norm_rope_kernel<__half, false>);
+  auto bf16 = single ? qk_norm_rope_kernel<__nv_bfloat16, true> : qk_norm_rope_kernel<__nv_bfloat16, false>;
+  auto fp16 = single ? qk_norm_rope_kernel<__half, true> : qk_norm_rope_kernel<__half, false>;
+  auto kernel = dtype == 0 ? bf16 : fp16;
   return launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), kRopeWarps * 32, 0, stream, p);
 }
 
@@ -144,7 +154,8 @@ int64_t attn_items(int64_t Tq, int64_t batch, int heads_q, int heads_kv) {
 // the partial rows' way through memory (together about as long as four steps of two tiles); an uneven last wave costs up
 // to one item's time.  So not where items are short, nor where there are so many waves that the last hardly counts.
 int attn_shares(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int sms) {
-  if (batch < 1 || Tq < 1 || Tk < 8 * kAtTile) return 0;
+  // (the sum of at most kMaxShares items' work has to fit an int)
+  if (batch < 1 || Tq < 1 || Tk < 8 * kAtTile || Tk > (1 << 28)) return 0;
   const int shares = sms < kMaxShares ? sms : kMaxShares;
   return attn_items(Tq, batch, heads_q, heads_kv) < 24 * static_cast<int64_t>(shares) ? shares : 0;
 }
@@ -217,6 +228,7 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
     if (ops[i].t <= 0 || ops[i].h <= 0 || ops[i].t >= (int64_t{1} << 38) || ops[i].h >= (int64_t{1} << 38))
       return CONVROT_ERR_SHAPE;
   }
+  if (rows_overlap(Tq, out_t, heads_q, out_h, D)) return CONVROT_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k) | reinterpret_cast<uintptr_t>(lse)) & 3u)
     return CONVROT_ERR_ALIGN;
   DeviceState* st = nullptr;

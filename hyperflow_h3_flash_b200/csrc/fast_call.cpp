@@ -38,8 +38,9 @@ int type_of(const at::Tensor& t) {
 // A [tokens, heads, head_dim] tensor with neighbouring channels, of the given type (-1: any of the two).
 const at::Tensor* heads(PyObject* o, int device, int type) {
   const at::Tensor* t = plain(o, device);
-  if (!t || t->dim() != 3 || t->stride(2) != 1 || t->size(1) > (1 << 16) || t->size(2) > 256 || type_of(*t) < 0 || (type >= 0 && type_of(*t) != type)) return nullptr;
-  return t;
+  if (!t || t->dim() != 3 || t->stride(2) != 1 || t->size(1) > (1 << 16) || t->size(2) > 256) return nullptr;
+  const int own = type_of(*t);
+  return own < 0 || (type >= 0 && own != type) ? nullptr : t;
 }
 
 at::Tensor fresh(const at::Tensor& t) {

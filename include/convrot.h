@@ -200,17 +200,19 @@ int convrot_silu(const void* x, void* y, int64_t n, void* stream);
  *                        the first R channels of y turned by table row t (fp32 [rows, >= R / 2, 2], ld_table pairs
  *                        apart, even; NULL: no rotation): pairs (2 j, 2 j + 1) if interleaved, else (j, j + R / 2);
  *                        (a, b) -> (a cos - b sin, b cos + a sin).  fp32 throughout, one rounding.  An output may be
- *                        its own input.  D a multiple of 8 up to 256; R a multiple of 8 (interleaved) or 16.
+ *                        its own input (same base and strides) and overlap nothing else, nor its rows each other.
+ *                        D a multiple of 8 up to 256; R a multiple of 8 (interleaved) or 16.
  * convrot_attention      out = softmax(scale q k^T + mask) v for `batch` sequences packed behind each other: sequence b
  *                        is rows [cu_q[b], cu_q[b + 1]) of q and out and [cu_k[b], cu_k[b + 1]) of k and v (device
  *                        arrays of batch + 1 non-decreasing offsets; both NULL: one sequence, batch 1).  Rows of no
  *                        sequence stay as they were.  Query head h reads key head h / (heads_q / heads_kv).  causal:
  *                        query i of lq sees keys up to i + lk - lq.  A row that sees no key gives zeros (lse
- *                        -infinity).  lse: fp32 [Tq, heads_q] natural log-sum-exp, or NULL.  fp32 scores, statistics
- *                        and sums; softmax weights rounded to dtype for the product with v.  D a multiple of 8 up to
- *                        128; heads_q / heads_kv <= 128; scale > 0.  The workspace (16-byte aligned, of
- *                        convrot_attention_workspace_size bytes on the current device, -1 for bad sizes; 0: none)
- *                        belongs to the call until its work is done.
+ *                        -infinity).  What a row does not see never reaches it, NaN and infinities included.  lse:
+ *                        fp32 [Tq, heads_q] natural log-sum-exp, or NULL.  fp32 scores, statistics and sums; softmax
+ *                        weights rounded to dtype for the product with v.  D a multiple of 8 up to 128; heads_q /
+ *                        heads_kv <= 128; scale > 0.  out overlaps no input, nor its rows each other.  The workspace
+ *                        (16-byte aligned, of convrot_attention_workspace_size bytes on the current device, -1 for bad
+ *                        sizes; 0: none; its content does not matter) belongs to the call until its work is done.
  */
 #define CONVROT_BF16 0
 #define CONVROT_FP16 1

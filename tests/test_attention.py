@@ -85,6 +85,17 @@ def test_the_joined_module_is_the_callable_of_an_attention_block():
     assert not any(p.requires_grad for p in core.parameters())
 
 
+def test_what_a_causal_row_does_not_see_does_not_reach_it_on_cpu():
+    q, k, v = _qkv(6, 9, 4, 2)
+    want = A.attention(q, k, v, causal=True)
+    v[7, 1, 3], v[8, 0, 0] = math.nan, math.inf
+    got = A.attention(q, k, v, causal=True)
+    assert got[4:, 2:, 3].isnan().all() and (got[5:, :2, 0] == math.inf).all()
+    got[4:, 2:, 3] = want[4:, 2:, 3]
+    got[5:, :2, 0] = want[5:, :2, 0]
+    torch.testing.assert_close(got, want, rtol=0, atol=1e-6)
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 
 
@@ -113,6 +124,9 @@ def test_attention_refuses_what_it_does_not_compute():
     refused("cu_k must be", cu_q=cu, cu_k=cu[None])
     refused("one length", cu_q=cu, cu_k=torch.tensor([0, 4, 9], dtype=torch.int32))
     refused("out must have", out=q[:3])
+    refused("one of the inputs", out=q)
+    same = _qkv(Tk=6, Hkv=4)
+    refused("one of the inputs", *same, out=same[2])
     refused("inference only", q.requires_grad_(), k, v)
     with torch.no_grad():
         assert not A.attention(q, k, v).requires_grad
@@ -171,6 +185,7 @@ def test_c_entries_refuse_bad_arguments_before_any_device_call(lib):  # noqa: F8
     assert attention(q=None) == attention(v=None) == attention(out=None) == lib.ERR_ARG
     assert attention(k_t=129) == attention(v_h=60) == attention(out=ctypes.c_void_p(4104)) == lib.ERR_ALIGN
     assert attention(lse=ctypes.c_void_p(4097)) == lib.ERR_ALIGN
+    assert attention(o_h=32) == attention(o_t=128) == attention(o_t=8, o_h=8) == lib.ERR_SHAPE  # rows that overlap
     assert attention(Tq=0) == attention(batch=0, cu_q=p, cu_k=p) == lib.OK
     assert L.convrot_attention_workspace_size(8, 8, 1, 3, 2, 64) == -1
     assert L.convrot_attention_workspace_size(0, 8, 1, 4, 2, 64) == 0
@@ -187,6 +202,7 @@ def test_c_entries_refuse_bad_arguments_before_any_device_call(lib):  # noqa: F8
     assert rope(dtype=3) == rope(norm=0, table=None) == rope(norm=0, wq=p) == rope(eps=-1.0) == lib.ERR_ARG
     assert rope(q=None) == rope(ko=None) == rope(eps=math.nan) == lib.ERR_ARG
     assert rope(q_t=257) == rope(ko_h=4) == rope(ld=33) == rope(wq=ctypes.c_void_p(4100)) == lib.ERR_ALIGN
+    assert rope(qo_h=0) == rope(ko_t=0) == rope(qo_t=128) == rope(ko_h=56) == lib.ERR_SHAPE  # rows that overlap
     assert rope(rows=0) == lib.OK
 
     def table(pos=p, kind=0, ld=2, rows=4, dims=(16, 16), theta=(1e4, 1e4), out=p):

@@ -498,6 +498,22 @@ def test_more_items_than_the_grid_has_sms():
     check(q, torch.cat([k, k, k])[:4500], torch.cat([v, v, v])[:4500], lens, lens, True)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("packed", [False, True])
+def test_items_that_fill_whole_waves(D, packed):
+    """Nothing is left over to be divided among the SMs."""
+    heads = torch.cuda.get_device_properties(0).multi_processor_count
+    q, k, v = qkv(40, 1100, heads, heads, D, seed=41)
+    check(q, k, v, [40], [1100], cu=packed)
+    assert _lib.lib().convrot_attention_workspace_size(40, 1100, 1, heads, heads, D) > 0
+
+
+def test_workspace_of_very_long_keys():
+    """Keys whose work, summed over the divided items, would pass 32 bits are not divided."""
+    size = _lib.lib().convrot_attention_workspace_size
+    assert size(1, 1 << 28, 1, 8, 1, 64) > 0 and size(1, (1 << 28) + 1, 1, 8, 1, 64) == 0
+
+
 def test_offsets_beyond_32_bits():
     """Queries, keys, values and outputs as columns of one wide buffer whose rows reach past 2^31 elements."""
     T, width = 34000, 65536
@@ -556,7 +572,7 @@ def test_refusals_on_the_gpu_leave_the_device_usable():
     wide = torch.empty(8, 2, 65, dtype=torch.bfloat16, device=DEV)
     for bad in (lambda: A.attention(q.float(), k.float(), v.float()), lambda: A.attention(wide[..., 1:], k, v),
                 lambda: A.attention(q, k.expand(8, 2, 64)[:, :1].expand(8, 2, 64), v), lambda: A.qk_norm_rope(q.float()),
-                lambda: A.qk_norm_rope(wide[..., 1:]), lambda: A.qk_norm_rope(q, k, q_out=k),
+                lambda: A.attention(q, k, v, out=q), lambda: A.qk_norm_rope(wide[..., 1:]), lambda: A.qk_norm_rope(q, k, q_out=k),
                 lambda: A.attention(q, k, v, cu_q=torch.zeros(2, dtype=torch.int32), cu_k=torch.zeros(2, dtype=torch.int32)),
                 lambda: A.rotary_table(torch.zeros(3, 2, dtype=torch.int16, device=DEV), (8, 8))):
         with pytest.raises(ValueError):
