@@ -1,7 +1,8 @@
-"""Builds ``libconvrot.so`` (the sm_100a kernels and their C ABI) in-tree with nvcc.
+"""Builds ``libconvrot.so`` (the sm_100a kernels and their C ABI) in-tree with nvcc, and ``_fast.so`` (the attention
+operators' common calls in compiled form) with the host compiler.
 
-``python -m hyperflow_h3_flash_b200.build`` or ``build()`` from Python. The library is written next to this file so
-that it travels with a copy of the repository; nothing is installed elsewhere.
+``python -m hyperflow_h3_flash_b200.build`` or ``build()`` from Python. Both are written next to this file so
+that they travel with a copy of the repository; nothing is installed elsewhere.
 """
 
 from __future__ import annotations
