@@ -469,14 +469,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x2(uint32_t taddr, uint32_t a, uint32_t b) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(a), "r"(b) : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld_32x32b_x2(uint32_t taddr, uint32_t& a, uint32_t& b) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(taddr) : "memory");
-}
-
 // Asks for the next CTA of the grid that has not been launched; the 16-byte answer arrives on `bar`.
 __device__ __forceinline__ void launch_cancel(uint32_t answer, uint32_t bar) {
   asm volatile(
@@ -553,7 +545,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
   const uint32_t v_need = bar0 + 8 * (2 * S + 12);      // a value tile with rows behind the sequence has arrived
   const uint32_t v_fixed = bar0 + 8 * (2 * S + 13);     // and those rows are cleared
   const uint32_t drain = bar0 + 8 * (2 * S + 14);
-  const uint32_t twin_ready = bar0 + 8 * (2 * S + 15);  // tile 1's part of a twin item is in TMEM
+  const uint32_t twin_ready = bar0 + 8 * (2 * S + 15);  // tile 1's o is in TMEM, its m and l in shared memory
   const uint32_t twin_done = bar0 + 8 * (2 * S + 16);   // and was read
   auto answer_full = [&](int i) { return bar0 + 8 * (2 * S + 17 + i); };
   auto item_full = [&](int i) { return bar0 + 8 * (2 * S + 19 + i); };
@@ -1117,9 +1109,11 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       }
       float w0 = 1.0f, w1 = 0.0f;  // of this tile's o, and of tile 1's in a twin item
       if (twin) {
-        if (i == 1) {  // m and l go where the scores were
-          tmem_st_32x32b_x2(s_addr, __float_as_uint(m), __float_as_uint(l));
-          tmem_st_wait();
+        // m and l go through the staging of tile 1's warp, which has no rows to write (not through TMEM: the next item's
+        // scores may already go where this one's were)
+        const uint32_t pass = smem_u32(staging + (4 + (warp & 3)) * Cfg::kStageOut) + lane * 8;
+        if (i == 1) {
+          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(pass), "f"(m), "f"(l) : "memory");
           tc_fence_before();
           __syncwarp();
           if (lane == 0) bar_arrive(twin_ready);
@@ -1132,10 +1126,8 @@ __global__ void __launch_bounds__(kAtThreads, 1)
         twin_phase ^= 1;
         __syncwarp();
         tc_fence_after();
-        uint32_t a, b;
-        tmem_ld_32x32b_x2(s_addr + 128, a, b);
-        tmem_ld_wait();
-        const float m1 = __uint_as_float(a), l1 = __uint_as_float(b);
+        float m1, l1;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(m1), "=f"(l1) : "r"(pass) : "memory");
         const float top = max3(m, m1, m1);  // NaN if one is
         if (top != -CUDART_INF_F) {
           w0 = m == -CUDART_INF_F ? 0.0f : exp2_approx((m - top) * c2);

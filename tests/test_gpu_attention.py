@@ -154,6 +154,15 @@ def test_single_tokens_over_long_keys(lk, new):
     check(q, k, v, lq, lk, True)
 
 
+@pytest.mark.parametrize("D,heads,group,lk", [(64, 2, 64, [2582]), (104, 3, 4, [2560, 0]), (128, 12, 1, [1200] * 9),
+                                              (40, 5, 8, [300, 4000, 1, 700]), (128, 1, 127, [260] * 40)])
+def test_one_tile_items_behind_each_other(D, heads, group, lk):
+    """Items of a single query tile, several to a CTA: what one leaves on the chip is not touched by the next."""
+    for seed in range(8):
+        q, k, v = qkv(len(lk), sum(lk), heads * group, heads, D, torch.float16 if seed & 1 else torch.bfloat16, seed=seed)
+        check(q, k, v, [1] * len(lk), lk, causal=seed & 2 != 0)
+
+
 def test_scores_that_grow_and_shrink_along_the_keys():
     """Maxima that jump by far more than the lazy rescaling's step, up and down, and rows of equal scores."""
     q, k, v = qkv(200, 1500, 2, 2, 64, seed=6, spread=1.0)
