@@ -10,7 +10,7 @@
 // qk_norm_rope_kernel: for each head row x of q and k
 //   y = x * rsqrt(mean(x^2) + eps) * w,   (a, b) -> (a c - b s, b c + a s) for each pair of the first R channels,
 // all in fp32, rounded once to the output type.  Bound by HBM (each row read once, written once): 32760 tokens of 2 x 40
-// heads of 128 take 221 us, 6.1 TB/s (231 with pairs half the rotated width apart; a plain copy of the same bytes 205),
+// heads of 128 take 220 us, 6.2 TB/s (231 with pairs half the rotated width apart; a plain copy of the same bytes 205),
 // ncu sees the issue slots as the next bound.  A lane holds 8 neighbouring channels (one 16-byte load) or two such
 // pieces, so that both channels of a pair are always its own; a row lies in a power-of-two group of lanes, so the sum of
 // squares is a few shuffles and the statistics never touch memory.  A warp takes several rows of one token at once:
@@ -116,7 +116,7 @@ struct QkRopeParams {
   float eps, inv_D;
 };
 
-constexpr int kRopeRows = 4;  // 16-byte loads of a lane in flight
+constexpr int kRopeRows = 4;  // 16-byte loads of a lane in flight (2: 339 us instead of 220, 8: 262)
 constexpr int kRopeWarps = 2;
 
 template <class T>
@@ -254,52 +254,70 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_kernel(const __g
     }
   }
 
+  // (two rows of 16 channels a lane at once take 93 registers, and 245 us instead of 231)
+  constexpr int kBatch = INTERLEAVED ? kSteps : 1;  // rows whose shuffles overlap
 #pragma unroll
-  for (int r = 0; r < kSteps; ++r) {
-    uint64_t x[kRegs];
+  for (int r0 = 0; r0 < kSteps; r0 += kBatch) {
+    uint64_t x[kBatch][kRegs];
 #pragma unroll
-    for (int h = 0; h < CH; ++h) {
-      const uint32_t v[4] = {raw[r][h].x, raw[r][h].y, raw[r][h].z, raw[r][h].w};
+    for (int r = 0; r < kBatch; ++r)
 #pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        const float2 f = Pack16<T>::unpack(v[i]), g = Pack16<T>::unpack(v[i + 1]);
-        x[4 * h + i] = INTERLEAVED ? pack2(f.x, g.x) : pack2(f.x, f.y);
-        x[4 * h + i + 1] = INTERLEAVED ? pack2(f.y, g.y) : pack2(g.x, g.y);
-      }
-    }
-    if (p.norm) {
-      uint64_t s2 = 0;
+      for (int h = 0; h < CH; ++h) {
+        const uint4 u = raw[r0 + r][h];
+        const uint32_t v[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int i = 0; i < kRegs; ++i) s2 = fma2(x[i], x[i], s2);
-      const float2 s = unpack2(s2);
-      float sum = s.x + s.y;
-      for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float inv = rsqrtf(fmaf(sum, p.inv_D, p.eps));
-#pragma unroll
-      for (int i = 0; i < kRegs; ++i) x[i] = mul2(x[i], pack2(inv, inv));
-    }
-    float2 y[kRegs];
-    if (p.table && turns) {
-#pragma unroll
-      for (int i = 0; i < kRegs; ++i) y[i] = unpack2(fma2(x[i], mine[i], mul2(x[i ^ kPartner], other[i])));
-    } else {
-#pragma unroll
-      for (int i = 0; i < kRegs; ++i) y[i] = unpack2(mul2(x[i], mine[i]));
-    }
-#pragma unroll
-    for (int h = 0; h < CH; ++h)
-      if (here[h] && row0 + r * per < heads) {
-        uint32_t u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = 4 * h + i;
-          if (INTERLEAVED)
-            u[i] = (i & 1) ? Pack16<T>::pack(y[k - 1].y, y[k].y) : Pack16<T>::pack(y[k].x, y[k + 1].x);
-          else
-            u[i] = Pack16<T>::pack(y[k].x, y[k].y);
+        for (int i = 0; i < 4; i += 2) {
+          const float2 f = Pack16<T>::unpack(v[i]), g = Pack16<T>::unpack(v[i + 1]);
+          x[r][4 * h + i] = INTERLEAVED ? pack2(f.x, g.x) : pack2(f.x, f.y);
+          x[r][4 * h + i + 1] = INTERLEAVED ? pack2(f.y, g.y) : pack2(g.x, g.y);
         }
-        __stcs(reinterpret_cast<uint4*>(out + r * per * out_h + h * apart), make_uint4(u[0], u[1], u[2], u[3]));
       }
+    if (p.norm) {
+      float sum[kBatch];
+#pragma unroll
+      for (int r = 0; r < kBatch; ++r) {
+        uint64_t s2 = 0;
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) s2 = fma2(x[r][i], x[r][i], s2);
+        const float2 s = unpack2(s2);
+        sum[r] = s.x + s.y;
+      }
+      for (int o = lanes >> 1; o; o >>= 1)
+#pragma unroll
+        for (int r = 0; r < kBatch; ++r) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
+#pragma unroll
+      for (int r = 0; r < kBatch; ++r) {
+        const float inv = rsqrtf(fmaf(sum[r], p.inv_D, p.eps));
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) x[r][i] = mul2(x[r][i], pack2(inv, inv));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kBatch; ++r) {
+      float2 y[kRegs];
+      if (p.table && turns) {
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) y[i] = unpack2(fma2(x[r][i], mine[i], mul2(x[r][i ^ kPartner], other[i])));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) y[i] = unpack2(mul2(x[r][i], mine[i]));
+      }
+#pragma unroll
+      for (int h = 0; h < CH; ++h)
+        if (here[h] && row0 + (r0 + r) * per < heads) {
+          uint32_t u[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = 4 * h + i;
+            if (INTERLEAVED)
+              u[i] = (i & 1) ? Pack16<T>::pack(y[k - 1].y, y[k].y) : Pack16<T>::pack(y[k].x, y[k + 1].x);
+            else
+              u[i] = Pack16<T>::pack(y[k].x, y[k].y);
+          }
+          __stcs(reinterpret_cast<uint4*>(out + (r0 + r) * per * out_h + h * apart),
+                 make_uint4(u[0], u[1], u[2], u[3]));
+        }
+    }
   }
 }
 
