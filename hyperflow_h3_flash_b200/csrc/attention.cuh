@@ -84,7 +84,7 @@ struct AttnParams {
   // shares > 0: the items that do not fill a whole wave of `shares` CTAs are divided evenly by key tiles, and what is
   // not a whole item goes to part_o / part_lse, joined by attention_combine_kernel.
   int shares;
-  int* meta;        // [kMaxShares + 4]: shares in use, items, first item, prefix of the items' work
+  int* meta;        // [kMaxShares + 4]: shares in use, items, first item, all work, prefix of the items' work
   float* part_o;    // [2 shares, 256, D] normalised rows
   float* part_lse;  // [2 shares, 256] log2-sum-exp
   uint64_t wait_limit_ns;
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
             if (sh.shares == 0) sh.divide(p, walk, whole, lane);
             if (s == 0) {  // for the kernel that joins the parts
               for (int i = lane; i <= sh.items; i += 32) p.meta[4 + i] = sh.items ? pre[i] : 0;
-              if (lane == 0) p.meta[0] = sh.shares, p.meta[1] = sh.items, p.meta[2] = whole;
+              if (lane == 0) p.meta[0] = sh.shares, p.meta[1] = sh.items, p.meta[2] = whole, p.meta[3] = sh.total;
             }
             if (sh.total > 0 && s < sh.shares) {  // (without items, pre and units hold nothing)
 #pragma unroll 1
@@ -1273,34 +1273,31 @@ __global__ void __launch_bounds__(kAtThreads, 1)
 
 // Joins the parts of the items that were divided: o = sum_s w_s o_s with w_s = 2^(lse_s - m) / sum 2^(lse_s - m), in
 // the order of the shares.  Block (x, y): rows y, y + gridDim.y, ... (by eights) of the x-th divided item; one warp a
-// row.  The partial rows were just written and mostly come from L2.
+// row.  The partial rows were just written and mostly come from L2; what bounds it is the launch and three loads behind
+// each other (9 us of the 127 for 1560 queries x 5 heads over 32760 keys; with a walk over the shares for each item, and
+// the rows loaded behind their weights, 14).
 template <class T>
 __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_constant__ AttnParams p) {
   grid_wait();
   grid_release();
   const int lane = threadIdx.x & 31;
-  const int shares = p.meta[0], items = p.meta[1], whole = p.meta[2], x = blockIdx.x;
+  const int x = blockIdx.x;
+  const int shares = p.meta[0], items = p.meta[1], whole = p.meta[2], all = p.meta[3];
+  const int from = p.meta[4 + x], upto = p.meta[5 + x];
   // (the limits also hold if the first kernel gave up and left no plan)
-  if (x >= items || items >= kMaxShares || shares < 1 || shares > p.shares) return;
-  int* pre = p.meta + 4;
-  const AttnShares sh{pre, nullptr, items, pre[items], shares};
-  const int from = pre[x], upto = pre[x + 1];
+  if (x >= items || items >= kMaxShares || shares < 1 || shares > p.shares || all < 1) return;
   AttnWalk walk;
   AttnPlace a;
   if (!walk.find(p, whole + x, lane, a)) return;
-  const int unit = attn_unit(p, a);
-  // the edges that lie inside this item
-  int s = max(1, static_cast<int>(static_cast<int64_t>(from) * shares / max(sh.total, 1)));
-  int first = 0, last = -1;  // shares of the item, if it was divided
-  for (; s < shares && sh.place(s) < upto; ++s) {
-    const int e = sh.snap(sh.place(s), from, upto, unit);
-    if (e <= from || e >= upto) continue;
-    if (last < 0) first = s - 1;
-    last = s;
-  }
-  if (last < 0) return;
+  // The edges inside this item: place(s) = all s / shares in [from + 4, upto - 4] (AttnShares::snap).
+  const int64_t low = static_cast<int64_t>(from + 4) * shares, high = static_cast<int64_t>(upto - 3) * shares;
+  const int s0 = max(1, static_cast<int>((low + all - 1) / all));
+  const int last = min(shares - 1, static_cast<int>((high + all - 1) / all) - 1);
+  if (last < s0) return;  // one share has it all
+  const int first = s0 - 1;
   const int heads = p.heads_kv * p.group;
   const int rows = min(a.lq - a.pos, 2 * p.positions) * p.group;
+  const int c = lane * 4;
   for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
     const int position = r / p.group, head = r - position * p.group;
     const int tile = position >= p.positions ? 1 : 0;
@@ -1308,28 +1305,34 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_con
     auto slot = [&](int s) {  // the first part of an item is its share's last
       return (2 * static_cast<int64_t>(s) + (s == first ? 1 : 0)) * 256 + at;
     };
-    float m = -CUDART_INF_F;
-    for (int s = first + lane; s <= last; s += 32) m = max3(m, p.part_lse[slot(s)], p.part_lse[slot(s)]);
+    auto part = [&](int s) {  // (a part without keys holds zeros)
+      return s <= last && c < p.D ? *reinterpret_cast<const float4*>(p.part_o + slot(s) * p.D + c)
+                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    };
+    float4 f[4];  // on their way while the weights are found
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = part(first + k);
+    float z = first + lane <= last ? p.part_lse[slot(first + lane)] : -CUDART_INF_F;
+    float m = z;
+    for (int s = first + 32 + lane; s <= last; s += 32) m = max3(m, p.part_lse[slot(s)], p.part_lse[slot(s)]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       const float other = __shfl_xor_sync(0xffffffffu, m, o);
       m = max3(m, other, other);
     }
-    const int c = lane * 4;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float total = 0.0f;
-    for (int from = first; from <= last; from += 32) {  // a lane for each part's weight, four rows in flight
-      const float z = from + lane <= last ? p.part_lse[slot(from + lane)] : -CUDART_INF_F;
+    for (int b = first; b <= last; b += 32) {  // a lane for each part's weight
+      if (b > first) z = b + lane <= last ? p.part_lse[slot(b + lane)] : -CUDART_INF_F;
       const float mine = z == -CUDART_INF_F ? 0.0f : exp2f(z - m);
-      const int n = min(32, last - from + 1);
-#pragma unroll 4
-      for (int k = 0; k < n; ++k) {
-        const float w = __shfl_sync(0xffffffffu, mine, k);
-        total += w;
-        if (c < p.D) {  // (a part without keys holds zeros)
-          const float4 f = *reinterpret_cast<const float4*>(p.part_o + slot(from + k) * p.D + c);
-          acc.x = fmaf(w, f.x, acc.x), acc.y = fmaf(w, f.y, acc.y);
-          acc.z = fmaf(w, f.z, acc.z), acc.w = fmaf(w, f.w, acc.w);
+      for (int k = 0; k < 32 && b + k <= last; k += 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float w = __shfl_sync(0xffffffffu, mine, k + e);
+          total += w;
+          acc.x = fmaf(w, f[e].x, acc.x), acc.y = fmaf(w, f[e].y, acc.y);
+          acc.z = fmaf(w, f[e].z, acc.z), acc.w = fmaf(w, f[e].w, acc.w);
+          f[e] = part(b + k + 4 + e);
         }
       }
     }

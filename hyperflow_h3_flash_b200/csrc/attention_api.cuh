@@ -183,7 +183,7 @@ int attn_map(CUtensorMap* map, const void* base, int dtype, int D, int64_t heads
 
 template <class T, int NP, bool CAUSAL>
 int launch_attention(const DeviceState& st, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                     const AttnParams& p, int64_t items, cudaStream_t stream) {
+                     const AttnParams& p, int64_t items, int joined, cudaStream_t stream) {
   auto kernel = attention_kernel<T, NP, CAUSAL>;
   int ready = -1;
   int rc = cached_resident(reinterpret_cast<const void*>(kernel), &ready);
@@ -196,10 +196,10 @@ int launch_attention(const DeviceState& st, const CUtensorMap& tq, const CUtenso
   }
   rc = launch_overlapped(kernel, dim3(static_cast<unsigned>(items)), kAtThreads, AttnCfg<NP>::kSmemBytes, stream, tq, tk,
                          tv, p);
-  if (rc || p.shares == 0) return rc;
+  if (rc || joined == 0) return rc;
   // a warp for each row that an item has at most (few tokens have few)
   const int positions = p.Tq < 2 * p.positions ? p.Tq : 2 * p.positions;
-  return launch_overlapped(attention_combine_kernel<T>, dim3(p.shares, (positions * p.group + 7) / 8), 256, 0, stream, p);
+  return launch_overlapped(attention_combine_kernel<T>, dim3(joined, (positions * p.group + 7) / 8), 256, 0, stream, p);
 }
 
 int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v,
@@ -279,15 +279,18 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
                      kAtTile)))
     return rc;
   // An upper bound of the work items (the kernel finds their number; what is beyond it finds nothing).
-  const int64_t items = attn_items(Tq, batch, heads_q, heads_kv) + p.shares;
+  const int64_t whole = attn_items(Tq, batch, heads_q, heads_kv), items = whole + p.shares;
   if (items > INT32_MAX / 2) return CONVROT_ERR_SHAPE;
+  // Items of the divided last wave: known, or at most one short of a wave.
+  const int64_t last = !p.shares ? 0 : !cu_q ? whole % p.shares : whole < p.shares ? whole : p.shares - 1;
+  const int joined = static_cast<int>(last);
   auto launch = [&](auto type) {
     using T = decltype(type);
     if (D <= 64)
-      return causal ? launch_attention<T, 1, true>(*st, tq, tk, tv, p, items, stream)
-                    : launch_attention<T, 1, false>(*st, tq, tk, tv, p, items, stream);
-    return causal ? launch_attention<T, 2, true>(*st, tq, tk, tv, p, items, stream)
-                  : launch_attention<T, 2, false>(*st, tq, tk, tv, p, items, stream);
+      return causal ? launch_attention<T, 1, true>(*st, tq, tk, tv, p, items, joined, stream)
+                    : launch_attention<T, 1, false>(*st, tq, tk, tv, p, items, joined, stream);
+    return causal ? launch_attention<T, 2, true>(*st, tq, tk, tv, p, items, joined, stream)
+                  : launch_attention<T, 2, false>(*st, tq, tk, tv, p, items, joined, stream);
   };
   return dtype == 0 ? launch(__nv_bfloat16()) : launch(__half());
 }
