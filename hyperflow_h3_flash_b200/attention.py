@@ -28,6 +28,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _lib
+from .int8 import _written
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
@@ -248,6 +249,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
                None if table is None else table.data_ptr(), R // 2, R, interleaved)
     if rc:
         _lib.check(rc, "convrot_qk_norm_rope")
+    _written(q_out, k_out)
     return qo if k is None else (qo, ko)
 
 
@@ -325,7 +327,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
         if cu_q.shape != cu_k.shape:
             raise ValueError(f"cu_q and cu_k must have one length, got {cu_q.shape[0]} and {cu_k.shape[0]}")
         batch = cu_q.shape[0] - 1
-    out = _output(out, q, "out")
+    given, out = out, _output(out, q, "out")
     if Tq and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
         raise ValueError("out must not be one of the inputs")
     lse = torch.empty(Tq, Hq, dtype=torch.float32, device=q.device) if return_lse else None
@@ -349,6 +351,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
                None if lse is None else lse.data_ptr(), None if space is None else space.data_ptr(), size)
     if rc:
         _lib.check(rc, "convrot_attention")
+    _written(given)
     return out if lse is None else (out, lse)
 
 

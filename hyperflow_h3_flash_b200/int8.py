@@ -271,6 +271,19 @@ class Int8RotLinear(nn.Module):
         return (acc * sx * self.wscale[None, :]).to(torch.bfloat16)
 
 
+def _written(*tensors: Tensor | None) -> None:
+    """Counts a kernel's write into tensors that a caller gave, as torch's own in-place operations do: the kernels get
+    an address only, and ``Int8RotLinear._quantize`` recognises its last input by the tensor and its version.  An
+    inference tensor has no version, so the kept input goes."""
+    for t in tensors:
+        if t is None:
+            continue
+        if t.is_inference():
+            Int8RotLinear._last_input.clear()
+        else:
+            torch.autograd.graph.increment_version(t)
+
+
 def _stacked_down(peers: tuple) -> Tensor:
     """``[down_q; down_k; down_v]`` for layers joined by ``share_lowrank``, built once and rebuilt only when one of
     the weights is replaced, moved or modified in place (kept on the first layer, keyed by address and version)."""

@@ -587,3 +587,35 @@ def test_refusals_on_the_gpu_leave_the_device_usable():
         with pytest.raises(ValueError):
             bad()
     check(q, k, v, [8], [8], cu=False)
+
+
+# ------------------------------------------------------------------------------------------------ given outputs
+
+
+def _layer_that_keeps_its_input(width, group):
+    from hyperflow_h3_flash_b200 import int8 as I
+    from hyperflow_h3_flash_b200 import synthetic
+
+    layer = I.Int8RotLinear(width, 256, group)
+    synthetic.load_into(layer, synthetic.linear_weights(width, 256, bias=False, group=group))
+    layer.keep_input = True
+    return layer.to(DEV)
+
+
+@pytest.mark.parametrize("inference", [False, True])
+@pytest.mark.parametrize("view", [False, True])
+def test_a_buffer_that_is_written_again_is_quantised_again(view, inference):
+    """A layer with keep_input recognises its last input by the tensor and its version: writing into a given output
+    counts as torch's own in-place operations do, for the buffer and for a view of it that was kept."""
+    T, H, D = 96, 1 if not view else 2, 128
+    layer = _layer_that_keeps_its_input(H * D, 64)
+    with torch.inference_mode(inference):
+        q, k, v = qkv(T, T, H, H, D, seed=70)
+        buf = torch.zeros_like(q)
+        x = buf.view(T, H * D) if view else buf
+        for write in (lambda: A.attention(q, k, v, out=buf), lambda: A.qk_norm_rope(q, q_out=buf),
+                      lambda: A.qk_norm_rope(q, k, q_out=torch.empty_like(q), k_out=buf)):
+            before = layer(x)
+            write()
+            got = layer(x)
+            assert torch.equal(got, layer(x.clone())) and not torch.equal(got, before)
