@@ -603,6 +603,7 @@ def convrot_matmul(a: Tensor, b: Tensor, sa: Tensor, sb: Tensor, *, bias: Tensor
                                      up.stride(0) if up is not None else 0, r, M, N, Kp, _ptr(out), out.stride(0),
                                      _stream(a))
         _lib.check(rc, "convrot_gemm")
+        _written(out)
         return out
     ldy = -(-N // 8) * 8
     y = torch.empty(M, ldy, dtype=torch.bfloat16, device=a.device)

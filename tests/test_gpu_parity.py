@@ -825,3 +825,24 @@ def test_convrot_matmul_into_a_row_slice_equals_the_plain_result():
                 torch.empty(N, M, dtype=torch.bfloat16, device=DEV).t()):
         with pytest.raises(ValueError, match="out must be"):
             I.convrot_matmul(q, w.qweight, s, w.wscale, bias=w.bias, xa=xa, up=w.up, out=bad)
+
+
+def _keeps_its_input(width):
+    layer = I.Int8RotLinear(width, 256, 64)
+    synthetic.load_into(layer, synthetic.linear_weights(width, 256, bias=False, group=64))
+    layer.keep_input = True
+    return layer.to(DEV)
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_a_matmul_into_a_given_output_is_seen_by_keep_input(inference):
+    """convrot_matmul(out=) counts as a write of its output: a layer that kept the buffer quantises it again."""
+    M, K = 64, 256
+    layer, first = _keeps_its_input(K), _keeps_its_input(K)
+    with torch.inference_mode(inference):
+        buf = synthetic.activations(M, K, seed=5).to(DEV)
+        codes, scales = I.rotate_quant(synthetic.activations(M, K, seed=6).to(DEV), 64)
+        before = layer(buf)
+        I.convrot_matmul(codes, first.qweight, scales, first.wscale, out=buf)
+        got = layer(buf)
+        assert torch.equal(got, layer(buf.clone())) and not torch.equal(got, before)
