@@ -20,6 +20,8 @@ from collections.abc import Callable
 import torch
 from torch import Tensor
 
+from .int8 import Int8RotLinear
+
 
 class CapturedCall:
     """``fn(*inputs)`` recorded once into a CUDA graph and replayed per call.
@@ -52,6 +54,9 @@ class CapturedCall:
             if src.data_ptr() != dst.data_ptr():
                 dst.copy_(src, non_blocking=True)
         self.graph.replay()
+        # A replay writes its outputs, and whatever else the recorded call writes, without moving any tensor's version:
+        # a layer with keep_input must not take such a tensor for its unmodified last input.
+        Int8RotLinear._last_input.clear()
         return self.outputs
 
 

@@ -846,3 +846,19 @@ def test_a_matmul_into_a_given_output_is_seen_by_keep_input(inference):
         I.convrot_matmul(codes, first.qweight, scales, first.wscale, out=buf)
         got = layer(buf)
         assert torch.equal(got, layer(buf.clone())) and not torch.equal(got, before)
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_a_replayed_output_is_seen_by_keep_input(inference):
+    """A replay writes the same output tensors again: a layer that kept one quantises it again."""
+    from hyperflow_h3_flash_b200.graphs import CapturedCall
+
+    M, K = 64, 256
+    layer, first = _keeps_its_input(K), _keeps_its_input(K)
+    first.keep_input = False
+    with torch.inference_mode(inference):
+        a, b = (synthetic.activations(M, K, seed=s).to(DEV) for s in (7, 8))
+        call = CapturedCall(first, a)
+        before = layer(call(a))
+        got = layer(call(b))
+        assert torch.equal(got, layer(first(b))) and not torch.equal(got, before)
