@@ -41,9 +41,13 @@ class CapturedCall:
                 fn(*self.inputs)
         torch.cuda.current_stream(self.inputs[0].device).wait_stream(side)
         torch.cuda.synchronize(self.inputs[0].device)
+        # What a layer with keep_input kept from the warm-up must not stand in for work of the recorded call, nor the
+        # recorded call's buffers for work of a later one.
+        Int8RotLinear._last_input.clear()
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.outputs = fn(*self.inputs)
+        Int8RotLinear._last_input.clear()
 
     def __call__(self, *inputs: Tensor) -> Tensor | tuple[Tensor, ...]:
         if len(inputs) != len(self.inputs):

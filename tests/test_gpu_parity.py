@@ -862,3 +862,18 @@ def test_a_replayed_output_is_seen_by_keep_input(inference):
         before = layer(call(a))
         got = layer(call(b))
         assert torch.equal(got, layer(first(b))) and not torch.equal(got, before)
+
+
+def test_a_captured_layer_that_keeps_its_input_quantises_in_the_graph():
+    """The kept input of the warm-up runs is not taken over into the recorded call, nor the recorded one's out of it."""
+    from hyperflow_h3_flash_b200.graphs import CapturedCall
+
+    layer = _keeps_its_input(256)
+    a, b = (synthetic.activations(64, 256, seed=s).to(DEV) for s in (9, 10))
+    call = CapturedCall(layer, a)
+    got = call(b).clone()
+    assert torch.equal(got, layer(b))
+    assert torch.equal(layer(call.inputs[0]), got)
+    call.inputs[0].copy_(a)
+    call.graph.replay()
+    assert torch.equal(call.outputs, layer(a))
