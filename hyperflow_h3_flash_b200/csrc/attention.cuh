@@ -182,6 +182,7 @@ struct AttnWalk {
   int block = 0;
 
   __device__ __forceinline__ bool find(const AttnParams& p, int item, int lane, AttnPlace& a) {
+    if (item < 0) return false;
     const int span = 2 * p.positions;
     if (!p.cu_q) {
       a.q0 = a.k0 = 0;
@@ -1284,13 +1285,16 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_con
   const int x = blockIdx.x;
   const int shares = p.meta[0], items = p.meta[1], whole = p.meta[2], all = p.meta[3];
   const int from = p.meta[4 + x], upto = p.meta[5 + x];
-  // (the limits also hold if the first kernel gave up and left no plan)
+  // Where the first kernel gave up, or offsets of sequences that overlap made more items than the grid has CTAs, no plan
+  // was written and the workspace holds anything.  With these limits every such content leads either nowhere or to rows
+  // of a sequence: find() takes no item but the call's own, and parts beyond the workspace's are not read.
   if (x >= items || items >= kMaxShares || shares < 1 || shares > p.shares || all < 1) return;
+  if (whole < 0 || whole % p.shares != 0 || from < 0 || upto <= from || upto > all) return;
   AttnWalk walk;
   AttnPlace a;
   if (!walk.find(p, whole + x, lane, a)) return;
   // The edges inside this item: place(s) = all s / shares in [from + 4, upto - 4] (AttnShares::snap).
-  const int64_t low = static_cast<int64_t>(from + 4) * shares, high = static_cast<int64_t>(upto - 3) * shares;
+  const int64_t low = (int64_t{from} + 4) * shares, high = (int64_t{upto} - 3) * shares;
   const int s0 = max(1, static_cast<int>((low + all - 1) / all));
   const int last = min(shares - 1, static_cast<int>((high + all - 1) / all) - 1);
   if (last < s0) return;  // one share has it all

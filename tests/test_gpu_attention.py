@@ -619,3 +619,51 @@ def test_a_buffer_that_is_written_again_is_quantised_again(view, inference):
             write()
             got = layer(x)
             assert torch.equal(got, layer(x.clone())) and not torch.equal(got, before)
+
+
+# ------------------------------------------------------------------------------------------------ bounds
+
+
+def _guarded(rows, *rest, dtype, pad=512):
+    """A tensor in the middle of a buffer of sevens, and a check that the rows around it are as they were."""
+    buf = torch.full((rows + 2 * pad, *rest), 7.0, dtype=dtype, device=DEV)
+
+    def untouched():
+        return bool((buf[:pad] == 7).all() and (buf[pad + rows :] == 7).all())
+
+    return buf[pad : pad + rows], untouched
+
+
+def _attention_entry(q, k, v, cu_q, cu_k, causal, out, lse, space):
+    """convrot_attention itself, on a workspace of the caller's."""
+    P = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    (Tq, Hq, D), (Tk, Hkv, _) = q.shape, k.shape
+    return _lib.lib().convrot_attention(
+        P(q), *q.stride()[:2], P(k), *k.stride()[:2], P(v), *v.stride()[:2], P(cu_q), P(cu_k),
+        1 if cu_q is None else cu_q.numel() - 1, Tq, Tk, Hq, Hkv, D, 0, D**-0.5, causal, P(out), *out.stride()[:2], P(lse),
+        P(space), space.numel() * space.element_size(), torch.cuda.current_stream().cuda_stream)
+
+
+NO_PLAN = [  # shares, items, first item, all work, then the work before each item in equal steps of the last number
+    (0, 0, 0, 0, 0), (5, 100, -37, 4000, 40), (5, 100, -148, 4000, 40), (148, 147, 3, 4000, 20), (148, 147, 1 << 30, 9000, 60),
+    (148, 147, 148, 9000, 60), (148, 147, 2**31 - 2, 9000, 60), (1, 191, 0, 2**31 - 1, 10_000_000), (148, 147, 0, 9000, -60)]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("plan", NO_PLAN)
+def test_a_plan_that_was_never_written_leads_nowhere(plan, causal):
+    """Offsets of sequences that overlap, which the arrays must not hold, make more items than the grid has CTAs, and
+    the plan for the joining kernel is not written: whatever the workspace held, nothing outside the outputs is."""
+    T, heads = 1024, 20
+    q, k, v = qkv(T, T, heads, heads, 64, seed=80)
+    cu = torch.tensor([0, T] * 8, dtype=torch.int32, device=DEV)
+    size = _lib.lib().convrot_attention_workspace_size(T, T, 15, heads, heads, 64)
+    assert size > 0
+    space = torch.zeros(size // 4, dtype=torch.int32, device=DEV)
+    space[:4] = torch.tensor(plan[:4])
+    space[4:196] = torch.tensor([max(-(2**31), min(2**31 - 1, i * plan[4])) for i in range(192)])
+    out, out_kept = _guarded(T, heads, 64, dtype=torch.bfloat16)
+    lse, lse_kept = _guarded(T, heads, dtype=torch.float32)
+    assert _attention_entry(q, k, v, cu, cu, causal, out, lse, space) == 0
+    torch.cuda.synchronize()
+    assert out_kept() and lse_kept()
