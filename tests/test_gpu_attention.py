@@ -667,3 +667,18 @@ def test_a_plan_that_was_never_written_leads_nowhere(plan, causal):
     assert _attention_entry(q, k, v, cu, cu, causal, out, lse, space) == 0
     torch.cuda.synchronize()
     assert out_kept() and lse_kept()
+
+
+@pytest.mark.parametrize("cu", [[0, 5000, 2048], [-5, 1100, 2048], [1500, 20, 2048], [2**31 - 1, -(2**31), 2**31 - 1],
+                                [0, 2048, 0, 2048], [7, 7, 7]])
+def test_offsets_that_make_no_sense_write_nothing_outside(cu):
+    T = 2048
+    q, k, v = qkv(T, T, 4, 2, 64, seed=81)
+    cu = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    assert _lib.lib().convrot_attention_workspace_size(T, T, cu.numel() - 1, 4, 2, 64) > 0
+    for causal in (False, True):
+        for cu_q, cu_k in ((cu, cu), (cu, torch.full_like(cu, T)), (torch.linspace(0, T, cu.numel(), device=DEV).int(), cu)):
+            out, kept = _guarded(T, 4, 64, dtype=torch.bfloat16)
+            A.attention(q, k, v, cu_q=cu_q, cu_k=cu_k, causal=causal, out=out)
+            torch.cuda.synchronize()
+            assert kept()
