@@ -13,8 +13,8 @@ elements (slices of a fused projection go in as they are).  Sequences of a batch
 offsets on the device (``cu_q``, ``cu_k``: ``[batch + 1]``), which are read on the GPU only: no call synchronises.
 
 CUDA tensors run the kernels of ``libconvrot.so``; there is no other path on CUDA.  CPU tensors take plain torch
-operations in fp32, as the package's layers do.  Inference only, like the layers around them: an input that requires
-grad is refused while grad mode is on.
+operations in fp32, as the package's layers do.  Inference only, like the layers around them: an input or a given output
+that requires grad is refused while grad mode is on.
 """
 
 from __future__ import annotations
@@ -110,6 +110,7 @@ def rotary_table(positions: Tensor, axes: Sequence[int], *, theta: float | Seque
         table = fast.rotary_table(positions, axes, theta)
         if table is not None:
             return table
+    _no_grad(positions)
     axes = tuple(int(d) for d in axes)
     if not 1 <= len(axes) <= 8 or any(d <= 0 or d % 2 for d in axes) or sum(axes) > 256:
         raise ValueError(f"axes must be 1 to 8 even positive widths of at most 256 channels in all, got {axes}")
@@ -186,7 +187,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
         made = fast.qk_norm_rope(q, k, q_weight, k_weight, eps, norm, table, interleaved)
         if made is not None:
             return made
-    _no_grad(q, k, q_weight, k_weight)
+    _no_grad(q, k, q_weight, k_weight, table, q_out, k_out)
     (T, Hq, D), qs = _heads(q, "q")
     if k is not None:
         k_shape, ks = _heads(k, "k", q)
@@ -303,7 +304,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
         made = fast.attention(q, k, v, cu_q, cu_k, causal, scale, return_lse)
         if made is not None:
             return made
-    _no_grad(q, k, v)
+    _no_grad(q, k, v, out)
     (Tq, Hq, D), qs = _heads(q, "q")
     (Tk, Hkv, Dk), ks = _heads(k, "k", q)
     v_shape, vs = _heads(v, "v", q)

@@ -214,3 +214,18 @@ def test_c_entries_refuse_bad_arguments_before_any_device_call(lib):  # noqa: F8
     assert table(dims=(2,) * 9, theta=(1.0,) * 9) == lib.ERR_SHAPE
     assert table(pos=ctypes.c_void_p(4098)) == table(kind=3, pos=ctypes.c_void_p(4100)) == lib.ERR_ALIGN
     assert table(rows=0) == lib.OK
+
+
+def test_every_input_and_given_output_that_requires_grad_is_refused():
+    q, k, v = _qkv(5, 5)
+    table = A.rotary_table(torch.arange(5), (16,))
+    wants = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [lambda: A.attention(q, wants(k), v), lambda: A.attention(q, k, wants(v)), lambda: A.attention(q, k, v, out=wants(q)),
+             lambda: A.qk_norm_rope(q, wants(k)), lambda: A.qk_norm_rope(q, k, table=wants(table)),
+             lambda: A.qk_norm_rope(q, k, q_out=wants(q)), lambda: A.qk_norm_rope(q, k, k_out=wants(k)),
+             lambda: A.rotary_table(wants(torch.arange(5.0)), (16,)), lambda: A.rotary_table(wants(torch.ones(5, 2)), (8, 8))]
+    for call in calls:
+        with pytest.raises(ValueError, match="inference only"):
+            call()
+        with torch.no_grad():
+            call()

@@ -682,3 +682,23 @@ def test_offsets_that_make_no_sense_write_nothing_outside(cu):
             A.attention(q, k, v, cu_q=cu_q, cu_k=cu_k, causal=causal, out=out)
             torch.cuda.synchronize()
             assert kept()
+
+
+# ------------------------------------------------------------------------------------------------ derivatives
+
+
+def test_every_input_and_given_output_that_requires_grad_is_refused():
+    q, k, v = qkv(5, 5, 2, 2, 64, seed=82)
+    table, w = A.rotary_table(torch.arange(5, device=DEV), (64,)), torch.ones(64, device=DEV)
+    wants = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [lambda: A.attention(wants(q), k, v), lambda: A.attention(q, wants(k), v), lambda: A.attention(q, k, wants(v)),
+             lambda: A.attention(q, k, v, out=wants(q)), lambda: A.qk_norm_rope(wants(q)), lambda: A.qk_norm_rope(q, wants(k)),
+             lambda: A.qk_norm_rope(q, q_weight=wants(w)), lambda: A.qk_norm_rope(q, k, table=wants(table)),
+             lambda: A.qk_norm_rope(q, k, q_out=wants(q)), lambda: A.qk_norm_rope(q, k, k_out=wants(k)),
+             lambda: A.rotary_table(wants(torch.arange(5.0, device=DEV)), (16,)),
+             lambda: A.rotary_table(wants(torch.ones(5, 2, device=DEV)), (8, 8))]
+    for call in calls:
+        with pytest.raises(ValueError, match="inference only"):
+            call()
+        with torch.no_grad():
+            call()
