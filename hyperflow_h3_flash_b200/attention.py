@@ -14,7 +14,7 @@ offsets on the device (``cu_q``, ``cu_k``: ``[batch + 1]``), which are read on t
 
 CUDA tensors run the kernels of ``libconvrot.so``; there is no other path on CUDA.  CPU tensors take plain torch
 operations in fp32, as the package's layers do.  Inference only, like the layers around them: an input or a given output
-that requires grad is refused while grad mode is on.
+that requires grad is refused while grad mode is on, and one with a forward-mode tangent always.
 """
 
 from __future__ import annotations
@@ -26,6 +26,7 @@ from collections.abc import Sequence
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 
 from . import _lib
 from .int8 import _written
@@ -54,6 +55,10 @@ def _no_grad(*tensors: Tensor | None) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError("attention operators are inference only: use torch.no_grad() or detach the inputs")
+    if forward_ad._current_level >= 0:  # within a dual_level (no_grad() leaves forward mode on)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("attention operators are inference only: a forward-mode tangent would be lost")
 
 
 def _call(entry, device: torch.device, *args):

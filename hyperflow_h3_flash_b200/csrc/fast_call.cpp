@@ -28,6 +28,7 @@ const at::Tensor* plain(PyObject* o, int device) {
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda() || t.get_device() != device || t.layout() != at::kStrided) return nullptr;
   if (t.requires_grad() && c10::GradMode::is_enabled()) return nullptr;
+  if (t._fw_grad(/*level=*/0).defined()) return nullptr;  // a forward-mode tangent (there is one level)
   return &t;
 }
 

@@ -229,3 +229,21 @@ def test_every_input_and_given_output_that_requires_grad_is_refused():
             call()
         with torch.no_grad():
             call()
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    q, k, v = _qkv(5, 5)
+    table = A.rotary_table(torch.arange(5), (16,))
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: A.attention(dual(q), k, v), lambda: A.attention(q, k, dual(v)),
+                     lambda: A.qk_norm_rope(q, dual(k)), lambda: A.qk_norm_rope(q, q_weight=dual(torch.ones(16))),
+                     lambda: A.qk_norm_rope(q, table=dual(table)), lambda: A.rotary_table(dual(torch.arange(5.0)), (16,))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="tangent"):
+                    call()
+        A.attention(forward_ad.unpack_dual(dual(q)).primal, k, v)
+    with pytest.raises(ValueError, match="tangent"):
+        torch.func.jvp(lambda t: A.attention(t, k, v), (q,), (torch.ones_like(q),))

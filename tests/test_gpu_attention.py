@@ -702,3 +702,21 @@ def test_every_input_and_given_output_that_requires_grad_is_refused():
             call()
         with torch.no_grad():
             call()
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    q, k, v = qkv(5, 5, 2, 2, 64, seed=83)
+    table = A.rotary_table(torch.arange(5, device=DEV), (64,))
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: A.attention(dual(q), k, v), lambda: A.attention(q, dual(k), v), lambda: A.attention(q, k, dual(v)),
+                     lambda: A.qk_norm_rope(dual(q)), lambda: A.qk_norm_rope(q, dual(k)),
+                     lambda: A.qk_norm_rope(q, q_weight=dual(torch.ones(64, device=DEV))),
+                     lambda: A.qk_norm_rope(q, table=dual(table)), lambda: A.rotary_table(dual(torch.arange(5.0, device=DEV)), (16,)),
+                     lambda: A.rotary_table(dual(torch.ones(5, 2, device=DEV)), (8, 8))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="tangent"):
+                    call()
+        assert torch.equal(A.attention(forward_ad.unpack_dual(dual(q)).primal, k, v), A.attention(q, k, v))
