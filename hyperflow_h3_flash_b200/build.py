@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libconvrot.so")
@@ -66,17 +67,20 @@ def build_fast(force: bool = False, verbose: bool = False) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles the library, and the Python module beside it, if missing or older than their sources; returns the
-    library's path."""
-    build_fast(force, verbose)
-    if not force and not stale():
-        return LIB
-    tmp = LIB + ".tmp"
-    cmd = [nvcc(), *NVCC_FLAGS, "-o", tmp, os.path.join(HERE, "csrc", "convrot.cu")]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, LIB)
+    """Compiles the library if it is missing or older than its sources, then the Python module beside it; returns the
+    library's path.  The module is optional (without it the attention operators' calls take the way through ctypes): a
+    host that cannot compile it gets a warning."""
+    if force or stale():
+        tmp = LIB + ".tmp"
+        cmd = [nvcc(), *NVCC_FLAGS, "-o", tmp, os.path.join(HERE, "csrc", "convrot.cu")]
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, LIB)
+    try:
+        build_fast(force, verbose)
+    except (OSError, RuntimeError, ImportError, subprocess.CalledProcessError) as e:
+        warnings.warn(f"the compiled calls of the attention operators were not built: {e}", RuntimeWarning, stacklevel=2)
     return LIB
 
 

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
 
 import pytest
 import torch
@@ -247,3 +248,29 @@ def test_forward_mode_tangents_are_refused():
         A.attention(forward_ad.unpack_dual(dual(q)).primal, k, v)
     with pytest.raises(ValueError, match="tangent"):
         torch.func.jvp(lambda t: A.attention(t, k, v), (q,), (torch.ones_like(q),))
+
+
+# ------------------------------------------------------------------------------------------------ the compiled calls
+
+
+def test_the_library_is_built_where_the_compiled_calls_cannot_be(tmp_path, monkeypatch):
+    """The module of the compiled calls needs Python.h and torch's headers; the library does not, and comes first."""
+    import subprocess
+
+    from hyperflow_h3_flash_b200 import build
+
+    made = []
+
+    def run(cmd, check):
+        made.append(os.path.basename(cmd[0]))
+        if "-gencode" not in cmd:
+            raise subprocess.CalledProcessError(1, cmd)
+        with open(cmd[cmd.index("-o") + 1], "w"):
+            pass
+
+    monkeypatch.setattr(build, "LIB", str(tmp_path / "libconvrot.so"))
+    monkeypatch.setattr(build, "nvcc", lambda: "nvcc")
+    monkeypatch.setattr(build.subprocess, "run", run)
+    with pytest.warns(RuntimeWarning, match="compiled calls"):
+        assert build.build(force=True) == build.LIB
+    assert os.path.exists(build.LIB) and made == ["nvcc", os.path.basename(os.environ.get("CXX", "g++"))]
