@@ -21,14 +21,16 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.util
 import math
+import warnings
 from collections.abc import Sequence
 
 import torch
 from torch import Tensor, nn
 from torch.autograd import forward_ad
 
-from . import _lib
+from . import _lib, build
 from .int8 import _written
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
@@ -38,16 +40,22 @@ MAX_HEAD_DIM = 128  # of attention; qk_norm_rope takes heads up to 256
 
 @functools.cache
 def _fast_calls():
-    """The compiled form of the common calls (csrc/fast_call.cpp), or None if it was not built: it calls the same C
-    entries, and answers None to every call that is not plainly in order, which then takes the way below."""
+    """The compiled form of the common calls (csrc/fast_call.cpp), or None if it was not built for this Python and torch:
+    it calls the same C entries, and answers None to every call that is not plainly in order, which then takes the way
+    below."""
+    path = build.fast_path()
     try:
-        from . import _fast
-    except ImportError:
+        spec = importlib.util.spec_from_file_location(f"{__package__}._fast", path)
+        fast = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(fast)
+    except ImportError as e:
+        warnings.warn(f"attention operators without their compiled calls ({e}): short calls take about 10 us longer; build "
+                      f"with `python -m {__package__}.build`", RuntimeWarning, stacklevel=3)
         return None
     handle = _lib.lib()
     names = ("rotary_table", "qk_norm_rope", "attention", "attention_workspace_size")
-    _fast.init(*(ctypes.cast(getattr(handle, f"convrot_{name}"), ctypes.c_void_p).value for name in names))
-    return _fast
+    fast.init(*(ctypes.cast(getattr(handle, f"convrot_{name}"), ctypes.c_void_p).value for name in names))
+    return fast
 
 
 def _no_grad(*tensors: Tensor | None) -> None:

@@ -274,3 +274,26 @@ def test_the_library_is_built_where_the_compiled_calls_cannot_be(tmp_path, monke
     with pytest.warns(RuntimeWarning, match="compiled calls"):
         assert build.build(force=True) == build.LIB
     assert os.path.exists(build.LIB) and made == ["nvcc", os.path.basename(os.environ.get("CXX", "g++"))]
+
+
+def test_compiled_calls_of_another_torch_or_python_are_not_taken(monkeypatch):
+    """The module's file carries the versions that it was compiled for; without one of these the way through ctypes is
+    taken, and a warning says so."""
+    from hyperflow_h3_flash_b200 import build
+
+    mine = build.fast_path()
+    assert torch.__version__ in mine and os.path.dirname(mine) == build.HERE
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    assert build.fast_path() != mine and build.stale(build.fast_path(), [build.FAST_SOURCE])
+    with pytest.warns(RuntimeWarning, match="compiled calls"):
+        assert A._fast_calls.__wrapped__() is None
+
+
+def test_a_compiled_module_that_cannot_be_loaded_is_not_taken(monkeypatch, tmp_path):
+    from hyperflow_h3_flash_b200 import build
+
+    broken = tmp_path / "_fast.so"
+    broken.write_bytes(b"not a module")
+    monkeypatch.setattr(build, "fast_path", lambda: str(broken))
+    with pytest.warns(RuntimeWarning, match="compiled calls"):
+        assert A._fast_calls.__wrapped__() is None
