@@ -59,11 +59,13 @@ int rotary_table(const void* pos, int pos_type, int64_t ld_pos, int64_t rows, in
 
 // ------------------------------------------------------------------------------------------------ norm and rotation
 
-// Whether rows of D elements, a x b of them, may share an element (the stride of a single one does not count).
+// Whether rows of D elements, a x b of them, may share an element (the stride of a single one does not count): the rows
+// of the smaller stride have to lie side by side within the larger one, (n - 1) stride + D <= larger.
 bool rows_overlap(int64_t a, int64_t stride_a, int64_t b, int64_t stride_b, int D) {
   if (a <= 1) return b > 1 && stride_b < D;
   if (b <= 1) return stride_a < D;
-  return stride_a < stride_b ? stride_a < D || stride_b / a < stride_a : stride_b < D || stride_a / b < stride_b;
+  if (stride_a > stride_b) return rows_overlap(b, stride_b, a, stride_a, D);
+  return stride_a < D || (stride_b - D) / (a - 1) < stride_a;
 }
 
 int qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, void* q_out, int64_t qo_t, int64_t qo_h, int heads_q,

@@ -297,3 +297,30 @@ def test_a_compiled_module_that_cannot_be_loaded_is_not_taken(monkeypatch, tmp_p
     monkeypatch.setattr(build, "fast_path", lambda: str(broken))
     with pytest.warns(RuntimeWarning, match="compiled calls"):
         assert A._fast_calls.__wrapped__() is None
+
+
+def test_rows_of_an_output_may_end_where_the_buffer_does(lib):  # noqa: F811
+    """Outputs whose last row has no padding behind it do not overlap; one element less and they do.  (A misaligned
+    pointer ends each call behind that check.)"""
+    L = lib.lib()
+    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4104 - 6)
+
+    def attention(Tq, Hq, o_t, o_h):
+        return L.convrot_attention(p, 256, 64, p, 128, 64, p, 128, 64, None, None, 1, Tq, 8, Hq, 2, 64, 0, 0.125, 0, p, o_t,
+                                   o_h, odd, None, 0, None)
+
+    def rope(T, H, qo_t, qo_h, ko_t, ko_h):
+        return L.convrot_qk_norm_rope(p, 256, 64, p, qo_t, qo_h, H, p, 256, 64, p, ko_t, ko_h, H, T, 64, 0, 1, odd, None, 0,
+                                      1e-6, None, 0, 0, 1, None)
+
+    for a, b in ((3, 4), (2, 2), (7, 4), (8, 2)):
+        for tight in (72, 640, 1 << 20):
+            wide = (a - 1) * tight + 64
+            assert attention(a, b, tight, wide) == lib.ERR_ALIGN  # heads first
+            assert attention(a, b, tight, wide - 8) == lib.ERR_SHAPE
+            assert rope(a, b, tight, wide, tight, wide + 8) == lib.ERR_ALIGN
+            assert rope(a, b, tight, wide, tight, wide - 8) == rope(a, b, tight, wide - 8, tight, wide) == lib.ERR_SHAPE
+            wide = (b - 1) * tight + 64
+            assert attention(a, b, wide, tight) == lib.ERR_ALIGN  # tokens first
+            assert attention(a, b, wide - 8, tight) == lib.ERR_SHAPE
+    assert attention(1 << 29, 2, 1 << 37, 64) == lib.ERR_ALIGN and attention(1 << 29, 2, 1 << 37, 1 << 37) == lib.ERR_SHAPE
