@@ -623,6 +623,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       auto send = [&](const AttnItem& x) {
         const int at = sent % kItems;
         guard.wait(item_empty(at), ((sent / kItems) & 1) ^ 1);
+        if (uniform(guard.aborted())) return;  // the place may still be read: rows of one item, limits of another
         if (lane == 0) {
           int4* dst = reinterpret_cast<int4*>(item_smem + at);
           dst[0] = make_int4(x.q_row, x.left, x.k_row, x.keys);
