@@ -357,7 +357,8 @@ __device__ __forceinline__ V uniform(V v) {
   return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// Waits for a phase of the mbarrier at a shared address, without a result: past the time limit it raises the abort flag
+// Waits for a phase of the mbarrier at a shared address, without a result: when no key or value tile was asked for within
+// the time limit (an item may well take longer, and warps 10 and 11 wait for its last tiles) it raises the abort flag
 // (and the device error word) and returns, and so does every later wait after two failed tries (about 2 us), so that every
 // loop below runs to its end on whatever data there is, at a few microseconds a key tile, and only the TMA producer, which
 // must not pile up loads, looks at the flag.  A result would have to be voted on by the issuing warp at every step; that
@@ -388,13 +389,17 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {  // wi
 }
 
 struct AttnGuard {
-  uint32_t abort;  // shared address of the flag
+  uint32_t abort;  // shared address of the flag; behind it, the number of tiles asked for so far
   const AttnParams& p;
 
   __device__ __forceinline__ bool aborted() const {
     int v;
     asm volatile("ld.volatile.shared.s32 %0, [%1];" : "=r"(v) : "r"(abort) : "memory");
     return v != 0;
+  }
+
+  __device__ __forceinline__ void progress(uint32_t loads) const {
+    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort + 4), "r"(loads) : "memory");
   }
 
   __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) const {
@@ -417,10 +422,16 @@ struct AttnGuard {
   }
   __device__ __forceinline__ void slow(uint32_t bar, uint32_t parity) const {
     uint64_t since = 0;
+    uint32_t seen = 0;
     while (!bar_try(bar, parity)) {
       if (aborted()) return;
       const uint64_t now = globaltimer_ns();
-      if (since == 0) since = now;
+      uint32_t loads;
+      asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(loads) : "r"(abort + 4) : "memory");
+      if (since == 0 || loads != seen) {
+        since = now;
+        seen = loads;
+      }
       if (now - since > p.wait_limit_ns) {
         asm volatile("st.volatile.shared.s32 [%0], 1;" ::"r"(abort) : "memory");
         if (p.error_word) atomicCAS(p.error_word, 0, 6 /* CONVROT_ERR_TIMEOUT */);
@@ -563,7 +574,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       const bool by_warps = (c >= 8 && c < 12) || c == 15 || c == 16, by_readers = c >= 19 + kItems && c < 19 + 2 * kItems;
       mbar_init(&bars[b], by_warps ? 4 : by_readers ? kReaders : 1);
     }
-    *abort_flag = 0;
+    abort_flag[0] = abort_flag[1] = 0;  // and the progress behind it
     fence_mbarrier_init();
     tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
@@ -720,7 +731,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       send(over);
     } else if (warp == 9) {
       // -------------------------------------------------------------- TMA producer
-      uint32_t stage = 0, phase = 0, issued_mask = 0, issued_parity = 0;
+      uint32_t stage = 0, phase = 0, issued_mask = 0, issued_parity = 0, loads = 0;
       uint32_t q_count[2] = {0, 0};
       bool stop = false;
       while (next_item()) {
@@ -755,6 +766,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
             for (int c = 0; c < NP; ++c)
               tma_load_3d(ring + stage * Cfg::kTileBytes + c * kAtPanelBytes, value ? &tmap_v : &tmap_k, full, c * 64,
                           it.head, it.k_row + tile * kAtTile);
+            guard.progress(++loads);
             issued_mask |= 1u << stage;
             issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
             if (++stage == S) {

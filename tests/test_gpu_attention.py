@@ -720,3 +720,25 @@ def test_forward_mode_tangents_are_refused():
                 with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="tangent"):
                     call()
         assert torch.equal(A.attention(forward_ad.unpack_dual(dual(q)).primal, k, v), A.attention(q, k, v))
+
+
+# ------------------------------------------------------------------------------------------------ the wait limit
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_an_item_may_take_longer_than_the_wait_limit(causal):
+    """The limit of the device-side waits bounds a stall, not the work of an item: here every CTA has one item of 256 key
+    tiles (about 350 us), under a limit of 100 us."""
+    L = _lib.lib()
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    q, k, v = qkv(sms * 256, 32768, 1, 1, 64, seed=84)
+    want = A.attention(q, k, v, causal=causal)
+    torch.cuda.synchronize()
+    L.convrot_set_wait_limit_ns(100_000)
+    try:
+        got = A.attention(q, k, v, causal=causal)
+        torch.cuda.synchronize()
+        assert L.convrot_poll_error(None) == 0
+    finally:
+        L.convrot_set_wait_limit_ns(0)
+    assert torch.equal(got, want)
