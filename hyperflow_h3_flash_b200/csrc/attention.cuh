@@ -240,10 +240,12 @@ struct AttnShares {
   int* pre;
   uint8_t* units;
   int items, total, shares;
+  bool cut;  // some item is long enough to be divided
 
   // Fills pre and units for the items from number `first` on (the whole warp).
   __device__ __forceinline__ void divide(const AttnParams& p, const AttnWalk& walk, int first, int lane) {
     const int span = 2 * p.positions;
+    int longest = 0;
     total = 0;
     if (lane == 0) pre[0] = 0;
 #pragma unroll 1
@@ -278,6 +280,7 @@ struct AttnShares {
         base += all;
       }
       work = k + lane < items ? work : 0;
+      longest = max(longest, work);
       work = attn_scan(work, lane);
       if (k + lane < items) {
         pre[k + lane + 1] = total + work;
@@ -286,9 +289,10 @@ struct AttnShares {
       total += __shfl_sync(0xffffffffu, work, 31);
     }
     __syncwarp();
-    // A share of less than 8 units costs more than it saves, unless it is an item of its own.  (No two edges can fall on
-    // one step: they are at least two units apart.)
-    shares = max(1, min(p.shares, max(total / 8, min(items, total / 2))));
+    // A share of less than 8 units costs more than it saves, unless it is an item of its own: where no item can be cut
+    // (see snap) each is one share.  (Else no two edges can fall on one step: they are at least two units apart.)
+    cut = __reduce_max_sync(0xffffffffu, longest) >= 8;
+    shares = cut ? max(1, min(p.shares, max(total / 8, min(items, total / 2)))) : max(items, 1);
   }
   __device__ __forceinline__ int item_at(int x, int lane) const {  // the item that work unit x < total lies in
     int n = 0;
@@ -307,6 +311,7 @@ struct AttnShares {
   }
   __device__ __forceinline__ int edge(int s, int lane) const {
     if (s >= shares) return total;
+    if (!cut) return pre[s];
     const int x = place(s), i = item_at(x, lane);
     return snap(x, pre[i], pre[i + 1], units[i]);
   }
@@ -628,7 +633,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       AttnPlace a;
       const int items = attn_count(p, lane);
       const int whole = p.shares > 0 ? items / p.shares * p.shares : items;
-      AttnShares sh{pre, units, items - whole, 0, 0};
+      AttnShares sh{pre, units, items - whole, 0, 0, false};
       uint32_t sent = 0, asked = 0;
       bool brief = false;
       auto send = [&](const AttnItem& x) {

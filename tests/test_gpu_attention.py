@@ -742,3 +742,18 @@ def test_an_item_may_take_longer_than_the_wait_limit(causal):
     finally:
         L.convrot_set_wait_limit_ns(0)
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------ shares
+
+
+@pytest.mark.parametrize("D,causal", [(64, False), (128, True)])
+def test_short_items_of_many_requests(D, causal):
+    """Last items that are too short to be cut: each is a share of its own, beside requests of other lengths and with
+    one among them that is cut."""
+    for lk in ([40] * 100, [128] * 147, [300] * 120, [1 + 7 * i % 300 for i in range(140)], [5000] + [17] * 90,
+               [17] * 90 + [5000], [513] * 30 + [2000, 0, 3]):
+        lq = [1 + i % 3 for i in range(len(lk))]
+        q, k, v = qkv(sum(lq), sum(lk), 4, 1, D, seed=85 + len(lk))
+        check(q, k, v, lq, lk, causal)
+        check(*qkv(len(lk), sum(lk), 5, 5, D, seed=86 + len(lk)), [1] * len(lk), lk, causal)
