@@ -1308,14 +1308,15 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const __grid_con
   // of a sequence: find() takes no item but the call's own, and parts beyond the workspace's are not read.
   if (x >= items || items >= kMaxShares || shares < 1 || shares > p.shares || all < 1) return;
   if (whole < 0 || whole % p.shares != 0 || from < 0 || upto <= from || upto > all) return;
-  AttnWalk walk;
-  AttnPlace a;
-  if (!walk.find(p, whole + x, lane, a)) return;
-  // The edges inside this item: place(s) = all s / shares in [from + 4, upto - 4] (AttnShares::snap).
+  // The edges inside this item: place(s) = all s / shares in [from + 4, upto - 4] (AttnShares::snap).  Looked at before the
+  // item's sequence is searched for, which takes several loads: most items of many short requests are not divided.
   const int64_t low = (int64_t{from} + 4) * shares, high = (int64_t{upto} - 3) * shares;
   const int s0 = max(1, static_cast<int>((low + all - 1) / all));
   const int last = min(shares - 1, static_cast<int>((high + all - 1) / all) - 1);
   if (last < s0) return;  // one share has it all
+  AttnWalk walk;
+  AttnPlace a;
+  if (!walk.find(p, whole + x, lane, a)) return;
   const int first = s0 - 1;
   const int heads = p.heads_kv * p.group;
   const int rows = min(a.lq - a.pos, 2 * p.positions) * p.group;
