@@ -156,13 +156,14 @@ __device__ __forceinline__ void attn_place(const AttnParams& p, int local, AttnP
   a.pos = (p.causal ? nq - 1 - qt : qt) * span;
 }
 
-// Work of an item in units of one 128 x 128 tile: a step of a pair of tiles counts two.
+// Work of an item in units of one 128 x 128 tile: a step of a pair of tiles counts two.  An item has at least 7: its first
+// tile and its output take as long, and items that cannot be divided (AttnShares::snap) get a share each.
 __device__ __forceinline__ int attn_unit(const AttnParams& p, const AttnPlace& a) {
   return a.lq - a.pos > p.positions ? 2 : 1;
 }
 __device__ __forceinline__ int attn_work(const AttnParams& p, const AttnPlace& a) {
   const int n = max(attn_tiles(p, a, a.pos), attn_tiles(p, a, a.pos + p.positions));
-  return max(n, 1) * attn_unit(p, a);
+  return max(n * attn_unit(p, a), 7);
 }
 
 // Sum of v over the lanes up to this one.
@@ -240,12 +241,10 @@ struct AttnShares {
   int* pre;
   uint8_t* units;
   int items, total, shares;
-  bool cut;  // some item is long enough to be divided
 
   // Fills pre and units for the items from number `first` on (the whole warp).
   __device__ __forceinline__ void divide(const AttnParams& p, const AttnWalk& walk, int first, int lane) {
     const int span = 2 * p.positions;
-    int longest = 0;
     total = 0;
     if (lane == 0) pre[0] = 0;
 #pragma unroll 1
@@ -280,7 +279,6 @@ struct AttnShares {
         base += all;
       }
       work = k + lane < items ? work : 0;
-      longest = max(longest, work);
       work = attn_scan(work, lane);
       if (k + lane < items) {
         pre[k + lane + 1] = total + work;
@@ -289,10 +287,9 @@ struct AttnShares {
       total += __shfl_sync(0xffffffffu, work, 31);
     }
     __syncwarp();
-    // A share of less than 8 units costs more than it saves, unless it is an item of its own: where no item can be cut
-    // (see snap) each is one share.  (Else no two edges can fall on one step: they are at least two units apart.)
-    cut = __reduce_max_sync(0xffffffffu, longest) >= 8;
-    shares = cut ? max(1, min(p.shares, max(total / 8, min(items, total / 2)))) : max(items, 1);
+    // A share of less than 8 units costs more than it saves, unless it is an item of its own.  (No two edges can fall on
+    // one step: they are at least 7 units apart.)
+    shares = max(1, min(p.shares, max(total / 8, items)));
   }
   __device__ __forceinline__ int item_at(int x, int lane) const {  // the item that work unit x < total lies in
     int n = 0;
@@ -311,7 +308,6 @@ struct AttnShares {
   }
   __device__ __forceinline__ int edge(int s, int lane) const {
     if (s >= shares) return total;
-    if (!cut) return pre[s];
     const int x = place(s), i = item_at(x, lane);
     return snap(x, pre[i], pre[i + 1], units[i]);
   }
@@ -633,7 +629,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
       AttnPlace a;
       const int items = attn_count(p, lane);
       const int whole = p.shares > 0 ? items / p.shares * p.shares : items;
-      AttnShares sh{pre, units, items - whole, 0, 0, false};
+      AttnShares sh{pre, units, items - whole, 0, 0};
       uint32_t sent = 0, asked = 0;
       bool brief = false;
       auto send = [&](const AttnItem& x) {
