@@ -152,14 +152,40 @@ int64_t attn_items(int64_t Tq, int64_t batch, int heads_q, int heads_kv) {
   return q_tiles * heads_kv;
 }
 
-// CTAs that share the items of the last wave evenly; 0: every item is one CTA's.  Dividing costs a second launch and
-// the partial rows' way through memory (together about as long as four steps of two tiles); an uneven last wave costs up
-// to one item's time.  So not where items are short, nor where there are so many waves that the last hardly counts.
-int attn_shares(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int sms) {
+// CTAs that share the items of the last wave evenly; 0: every item is one CTA's.
+//
+// Dividing saves the time that CTAs without a last item would idle, an item's work times their share, and costs a second
+// launch, a later start of the next kernel and the partial rows' way through memory.  In half steps (one 128 x 128 tile,
+// about 0.8 us of a CTA) the fixed part measured 14 and each megabyte of partial rows about one:
+//   1 token, 8 heads, 1536 / 2048 / 4096 keys (saves 11 / 15 / 30, costs 14): 21.0 / 17.9 / 18.6 us divided, 16.2 / 19.5 /
+//     32.7 not;
+//   256 tokens, 40 heads, 2048 / 4096 / 8192 keys (23 / 47 / 93, 39): 34.0 / 44.4 / 62.4 divided, 32.2 / 58.3 / 109.6 not;
+//   700 tokens, 40 heads, 1024 / 8192 keys, 120 items for 148 CTAs (3 / 24, 49): 48.9 / 157.5 divided, 21.4 / 140.0 not;
+//   4.3 waves of 40 heads, 2048 / 4096 / 32760 keys (22 / 43 / 346, 40): 173.9 / 310.9 / 2236 divided, 165.7 / 320.2 / 2453
+//     not; beyond 24 waves the difference is within 1 % either way.
+// The offsets of several sequences are not known here: any of them may be the long one, and may come last.  A sequence of
+// eight times the mean is reckoned with, and CTAs that would idle all the while.  Single tokens, 8 heads, divided / not:
+// 147 requests of 128 keys 26 / 10.6 us, 16 of 2000 keys 39.7 / 28.4, one of 32768 behind 63 of 100 keys 81 / 272.
+int attn_shares(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int D, int sms) {
   // (the sum of at most kMaxShares items' work has to fit an int)
   if (batch < 1 || Tq < 1 || Tk < 8 * kAtTile || Tk > (1 << 28)) return 0;
-  const int shares = sms < kMaxShares ? sms : kMaxShares;
-  return attn_items(Tq, batch, heads_q, heads_kv) < 24 * static_cast<int64_t>(shares) ? shares : 0;
+  const int shares = sms < kMaxShares ? sms : kMaxShares, group = heads_q / heads_kv;
+  const int64_t items = attn_items(Tq, batch, heads_q, heads_kv);
+  if (items >= 24 * static_cast<int64_t>(shares)) return 0;
+  auto longest = [&](int64_t all) {
+    const int64_t eightfold = 8 * ((all + batch - 1) / batch);
+    return eightfold < all ? eightfold : all;
+  };
+  const int64_t last = batch == 1 ? items % shares : items < shares ? items : shares - 1;
+  // (one sequence whose items fill whole waves: nothing is left to divide and nothing is launched for it, unless offsets
+  // make it shorter)
+  if (last == 0) return shares;
+  const int64_t rows = longest(Tq) * group, tile_rows = kAtTile / group * group;
+  const int64_t units = (longest(Tk) + kAtTile - 1) / kAtTile * (rows > tile_rows ? 2 : 1);
+  const int64_t idle = batch == 1 ? shares - last : shares;
+  const int64_t cuts = units * last / 8 < shares ? units * last / 8 : shares;
+  const int64_t part_bytes = (cuts + last) * (rows < 2 * tile_rows ? rows : 2 * tile_rows) * D * 4;
+  return units * idle > (14 + part_bytes / 1000000) * shares ? shares : 0;
 }
 
 size_t attn_workspace(int shares, int D) {
@@ -237,7 +263,7 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
   if ((rc = device_state(&st))) return rc;
   AttnParams p;
   memset(&p, 0, sizeof(p));
-  p.shares = attn_shares(Tq, Tk, batch, heads_q, heads_kv, st->sms);
+  p.shares = attn_shares(Tq, Tk, batch, heads_q, heads_kv, D, st->sms);
   if (p.shares > 0) {
     if (!workspace || workspace_bytes < attn_workspace(p.shares, D)) return CONVROT_ERR_ARG;
     if (!aligned16(workspace)) return CONVROT_ERR_ALIGN;

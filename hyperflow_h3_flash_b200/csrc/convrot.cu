@@ -1039,7 +1039,7 @@ int64_t convrot_attention_workspace_size(int64_t Tq, int64_t Tk, int64_t batch, 
   if (Tq == 0 || batch == 0) return 0;
   DeviceState* st = nullptr;
   if (device_state(&st)) return -1;
-  return static_cast<int64_t>(attn_workspace(attn_shares(Tq, Tk, batch, heads_q, heads_kv, st->sms), D));
+  return static_cast<int64_t>(attn_workspace(attn_shares(Tq, Tk, batch, heads_q, heads_kv, D, st->sms), D));
 }
 
 int convrot_attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, const void* v,
