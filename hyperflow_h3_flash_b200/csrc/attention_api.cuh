@@ -236,7 +236,8 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
               int64_t out_h, float* lse, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   int rc = attn_check(Tq, Tk, batch, heads_q, heads_kv, D);
   if (rc) return rc;
-  if (dtype < 0 || dtype > 1 || !(scale > 0.0f) || !(scale < 3e38f)) return CONVROT_ERR_ARG;
+  const float scale_log2 = scale * 1.4426950408889634f;  // what the kernel multiplies with
+  if (dtype < 0 || dtype > 1 || !(scale > 0.0f) || !isfinite(scale_log2)) return CONVROT_ERR_ARG;
   if ((cu_q == nullptr) != (cu_k == nullptr) || (!cu_q && batch != 1)) return CONVROT_ERR_ARG;
   if (Tq == 0 || batch == 0) return CONVROT_OK;
   if (!q || !out || (Tk > 0 && (!k || !v))) return CONVROT_ERR_ARG;
@@ -281,7 +282,7 @@ int attention(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_
   p.D = D;
   p.positions = kAtTile / p.group;
   p.group_inverse = (65536 + p.group - 1) / p.group;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   p.causal = causal ? 1 : 0;
   // Causal items go out longest first; over as many heads at once as keep their keys and values in L2, so that the
   // last ones are short.

@@ -324,3 +324,17 @@ def test_rows_of_an_output_may_end_where_the_buffer_does(lib):  # noqa: F811
             assert attention(a, b, wide, tight) == lib.ERR_ALIGN  # tokens first
             assert attention(a, b, wide - 8, tight) == lib.ERR_SHAPE
     assert attention(1 << 29, 2, 1 << 37, 64) == lib.ERR_ALIGN and attention(1 << 29, 2, 1 << 37, 1 << 37) == lib.ERR_SHAPE
+
+
+def test_a_scale_that_overflows_in_units_of_log2_is_refused(lib):  # noqa: F811
+    """The kernel takes scores times scale * log2(e), which has to be finite in fp32.  (A misaligned pointer ends the calls
+    with a good scale.)"""
+    L = lib.lib()
+    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4098)
+
+    def attention(scale):
+        return L.convrot_attention(p, 256, 64, p, 128, 64, p, 128, 64, None, None, 1, 8, 8, 4, 2, 64, 0, scale, 0, p, 256, 64,
+                                   odd, None, 0, None)
+
+    assert attention(2.3e38) == attention(1e-40) == attention(1.0) == lib.ERR_ALIGN
+    assert attention(2.4e38) == attention(2.9e38) == attention(3.4e38) == lib.ERR_ARG
