@@ -8,9 +8,10 @@ The reference leaves these steps to diffusers (called from chunk_block, src/hype
 * ``attention``: softmax attention over sequences packed behind each other, grouped heads, causal or not;
 * ``QKNormAttention``: the three joined, with the norms' weights: the callable for ``attention_block_linears``.
 
-The layout is ``[tokens, heads, head_dim]``, bf16 or fp16, with any token and head strides that are multiples of 8
-elements (slices of a fused projection go in as they are).  Sequences of a batch are packed along the tokens with int32
-offsets on the device (``cu_q``, ``cu_k``: ``[batch + 1]``), which are read on the GPU only: no call synchronises.
+The layout is ``[tokens, heads, head_dim]``, bf16 or fp16, with any token and head strides that are positive multiples of
+8 elements (slices of a fused projection go in as they are; heads that ``expand`` repeats do not: give them once, as
+grouped heads).  Sequences of a batch are packed along the tokens with int32 offsets on the device (``cu_q``, ``cu_k``:
+``[batch + 1]``), which are read on the GPU only: no call synchronises.
 
 CUDA tensors run the kernels of ``libconvrot.so``; there is no other path on CUDA.  CPU tensors take plain torch
 operations in fp32, as the package's layers do.  Inference only, like the layers around them: an input or a given output
@@ -305,6 +306,9 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
     * ``cu_q`` / ``cu_k`` (int32 ``[batch + 1]``, non-decreasing, on the device): sequence b is rows ``cu_q[b]:cu_q[b + 1]``
       of q and ``cu_k[b]:cu_k[b + 1]`` of k and v; None: one sequence.  Rows of no sequence (padding behind the last one)
       are not written: they keep what ``out`` held.
+    * A cache with room to grow: its rows that are not filled yet are a sequence without a query (``cu_q`` repeats its
+      offset, ``cu_k`` spans them); what they hold reaches no row.  With m caches of ``room`` rows and n[i] filled,
+      ``cu_k`` is ``[0, n[0], room, room + n[1], 2 * room, ...]`` and ``cu_q`` ``[0, 1, 1, 2, 2, ...]`` for a token each.
     * ``causal``: query i of lq sees the keys up to ``i + lk - lq`` (the last query sees all of them), so a prompt, a
       chunk behind a cache and a single new token are the same call.
     * A query that sees no key gives zeros (and ``-inf`` in the log-sum-exp).

@@ -782,3 +782,28 @@ def test_which_calls_are_divided():
             (4096, 4096, 1, 40, 40, True), (32760, 32760, 1, 5, 5, True), (32760, 333, 1, 40, 40, False),
             (147, 147 * 128, 147, 8, 1, False), (64, 63 * 100 + 32768, 64, 40, 8, True), (17, 333, 1, 8, 8, False)):
         assert (size(Tq, Tk, batch, hq, hkv, 128) > 0) == divided, (Tq, Tk, batch, hq, hkv)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_caches_with_room_to_grow(dtype):
+    """Rows of a cache that are not filled yet, given as sequences without a query: whatever they hold reaches nobody."""
+    room, filled = 640, [1, 640, 300, 129, 511]
+    k, v = (_randn(room * len(filled), 2, 128, seed=s, dtype=dtype) for s in (88, 89))
+    lq, lk = [], []
+    for i, n in enumerate(filled):
+        lq += [1, 0]
+        lk += [n, room - n]
+        for t in (k, v):
+            t[i * room + n : (i + 1) * room] = math.nan if i % 2 else math.inf
+    q = _randn(len(filled), 10, 128, seed=90, dtype=dtype)
+    for causal in (False, True):
+        got = A.attention(q, k, v, cu_q=_cu(lq), cu_k=_cu(lk), causal=causal)
+        keep = torch.cat([torch.arange(i * room, i * room + n, device=DEV) for i, n in enumerate(filled)])
+        want, _, bound, _ = reference(q, k[keep], v[keep], [1] * len(filled), filled, causal, 128**-0.5)
+        assert ((got.double() - want).abs() <= bound).all()
+    # the next token of each: the offsets move, the cache stays
+    for i, n in enumerate(filled):
+        if n < room:
+            k[i * room + n], v[i * room + n] = 0.5, 2.0
+    lk = [x for n in filled for x in (min(n + 1, room), room - min(n + 1, room))]
+    assert torch.isfinite(A.attention(q, k, v, cu_q=_cu(lq), cu_k=_cu(lk), causal=True)).all()
