@@ -338,3 +338,18 @@ def test_a_scale_that_overflows_in_units_of_log2_is_refused(lib):  # noqa: F811
 
     assert attention(2.3e38) == attention(1e-40) == attention(1.0) == lib.ERR_ALIGN
     assert attention(2.4e38) == attention(2.9e38) == attention(3.4e38) == lib.ERR_ARG
+
+
+def test_outputs_of_the_norm_must_not_be_the_other_ones_memory_on_cpu_either():
+    """As on the GPU: q's output over k's input (or both outputs in one place) would change what the other half reads."""
+    q, k, _ = _qkv(5, 5, 4, 4)
+    kept = k.clone()
+    for kw in ({"q_out": k}, {"k_out": q}, {"q_out": q, "k_out": q}):
+        with pytest.raises(ValueError, match="each other"):
+            A.qk_norm_rope(q, k, **kw)
+    with pytest.raises(ValueError, match="each other"):
+        A.qk_norm_rope(q, q, q_out=q, k_out=q)
+    assert torch.equal(k, kept)
+    want = A.qk_norm_rope(q, k)
+    got = A.qk_norm_rope(q, k, q_out=q, k_out=k)
+    assert got[0] is q and got[1] is k and all(torch.equal(a, b) for a, b in zip(got, want))
