@@ -807,3 +807,96 @@ def test_caches_with_room_to_grow(dtype):
             k[i * room + n], v[i * room + n] = 0.5, 2.0
     lk = [x for n in filled for x in (min(n + 1, room), room - min(n + 1, room))]
     assert torch.isfinite(A.attention(q, k, v, cu_q=_cu(lq), cu_k=_cu(lk), causal=True)).all()
+
+
+# ------------------------------------------------------------------------------------------------ more ways of use
+
+
+def test_captured_with_a_fork_a_copy_and_changing_offsets():
+    """One graph with a copied input, a branch on a second stream that joins again, and offsets that move between replays."""
+    T, Tk, H, D = 96, 4096, 4, 128
+    q, k, v = qkv(T, Tk, H, H, D, seed=91)
+    table = A.rotary_table(torch.arange(T, device=DEV), (D,))
+    cu_q, cu_k = _cu([40, 56]), _cu([4000, 96])
+    staged = torch.empty_like(q)
+
+    def call():
+        main, side = torch.cuda.current_stream(), streams[0]
+        staged.copy_(q)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            other = A.attention(staged, k, v, causal=True)
+        turned = A.qk_norm_rope(staged, table=table)
+        packed = A.attention(turned, k, v, cu_q=cu_q, cu_k=cu_k)
+        main.wait_stream(side)
+        return other, A.attention(A.qk_norm_rope(other, table=table), k, v), packed
+
+    streams = [torch.cuda.Stream()]
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for seed, lens in ((92, [(40, 56), (4000, 96)]), (93, [(1, 95), (1, 4095)]), (94, [(96, 0), (4096, 0)])):
+        q.copy_(_randn(T, H, D, seed=seed, dtype=q.dtype))
+        for cu, length in zip((cu_q, cu_k), lens):
+            cu.copy_(_cu(list(length)))
+        graph.replay()
+        torch.cuda.synchronize()
+        first = [t.clone() for t in got]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+        assert all(torch.equal(a, b) for a, b in zip(first, call()))
+
+
+def test_calls_from_several_threads_at_once():
+    import threading
+
+    cases = [(qkv(1 + 64 * i, 3000 + i, 4, 2, 64 + 64 * (i % 2), seed=95 + i), i % 2 == 0) for i in range(4)]
+    want = [A.attention(*c, causal=causal) for c, causal in cases]
+    tables = [A.rotary_table(torch.arange(c[0].shape[0], device=DEV), (64,)) for c, _ in cases]
+    turned = [A.qk_norm_rope(c[0], table=t) for (c, _), t in zip(cases, tables)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        (c, causal), stream = cases[i], torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for n in range(50):
+                out = torch.empty_like(c[0]) if n % 2 else None
+                got, rot = A.attention(*c, causal=causal, out=out), A.qk_norm_rope(c[0], table=tables[i])
+                stream.synchronize()
+                if not (torch.equal(got, want[i]) and torch.equal(rot, turned[i])):
+                    wrong.append((i, n))
+            stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_one_module_for_all_blocks_of_a_pass():
+    """The module's table and offsets serve every block, q and k of each are turned in place, and a replay of the captured
+    pass on new inputs gives what the calls give."""
+    T, H, D = 200, 4, 128
+    core = A.QKNormAttention(D, causal=True).to(DEV)
+    core.set_sequences(A.rotary_table(torch.arange(T, device=DEV), (D,)), _cu([150, 0, 50]))
+
+    def blocks(q, k, v):
+        for _ in range(3):
+            o = core(q.clone(), k.clone(), v)
+            q, k, v = o, q + o, v + o
+        return o
+
+    from hyperflow_h3_flash_b200.graphs import CapturedCall
+
+    call = CapturedCall(blocks, *qkv(T, T, H, H, D, seed=99))
+    for seed in (100, 101):
+        args = qkv(T, T, H, H, D, seed=seed)
+        kept = [t.clone() for t in args]
+        assert torch.equal(call(*args), blocks(*args))
+        assert all(torch.equal(a, b) for a, b in zip(args, kept))

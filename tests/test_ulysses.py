@@ -122,3 +122,37 @@ def test_peer_exchange_setup_failure_reaches_every_rank(tmp_path):
     assert all(not p.is_alive() for p in ctx.processes)
     for rank in range(world):
         assert "could not export" in torch.load(f"{tmp_path / 'out'}.{rank}")
+
+
+def _worker_joined_module(rank, world, store_path, out_path):
+    from hyperflow_h3_flash_b200 import attention as A
+
+    _init(rank, world, store_path)
+    try:
+        M, heads, d = 24, 4, 16
+        g = torch.Generator().manual_seed(3)
+        full = torch.randn(M, heads * d, generator=g)
+        w = [torch.randn(heads * d, heads * d, generator=g) / 8 for _ in range(4)]
+        layers = [lambda t, w=w_: t @ w for w_ in w]
+        core = A.QKNormAttention(d, causal=True, dtype=torch.float32)
+        core.norm_q.weight.copy_(torch.linspace(0.5, 2, d))
+        # all tokens of this rank's heads are here after the exchange: the table and the sequences are the whole batch's
+        table, cu = A.rotary_table(torch.arange(M), (d,)), torch.tensor([0, 10, 10, 17, M], dtype=torch.int32)
+        core.set_sequences(table, cu)
+        out = ulysses.attention_block_linears(ulysses.shard_rows(full, world, rank), *layers, heads, attention=core)
+        q, k, v = ((full @ w_).view(M, heads, d) for w_ in w[:3])
+        q, k = A.qk_norm_rope(q, k, q_weight=core.norm_q.weight, k_weight=core.norm_k.weight, table=table)
+        ref = A.attention(q, k, v, cu_q=cu, cu_k=cu, causal=True).reshape(M, -1) @ w[3]
+        # half the rows may take another order of sums: three products of 64 terms below 10, 3 * 64 * 10 * 2^-24 together
+        torch.save({"same": torch.allclose(out, ulysses.shard_rows(ref, world, rank), rtol=0, atol=1.2e-4)},
+                   f"{out_path}.{rank}")
+    finally:
+        dist.destroy_process_group()
+
+
+def test_joined_attention_module_on_two_cpu_ranks(tmp_path):
+    world = 2
+    out = tmp_path / "out"
+    mp.spawn(_worker_joined_module, args=(world, str(tmp_path / "store"), str(out)), nprocs=world, join=True)
+    for rank in range(world):
+        assert torch.load(f"{out}.{rank}") == {"same": True}, rank
