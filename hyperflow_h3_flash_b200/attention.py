@@ -24,6 +24,7 @@ import ctypes
 import functools
 import importlib.util
 import math
+import numbers
 import warnings
 from collections.abc import Sequence
 
@@ -128,7 +129,7 @@ def rotary_table(positions: Tensor, axes: Sequence[int], *, theta: float | Seque
     axes = tuple(int(d) for d in axes)
     if not 1 <= len(axes) <= 8 or any(d <= 0 or d % 2 for d in axes) or sum(axes) > 256:
         raise ValueError(f"axes must be 1 to 8 even positive widths of at most 256 channels in all, got {axes}")
-    thetas = [float(theta)] * len(axes) if isinstance(theta, (int, float)) else [float(v) for v in theta]
+    thetas = [float(theta)] * len(axes) if isinstance(theta, numbers.Real) else [float(v) for v in theta]
     if len(thetas) != len(axes) or any(not (v > 0 and math.isfinite(v)) for v in thetas):
         raise ValueError(f"theta must be positive, one value or one per axis, got {theta!r}")
     if positions.dim() == 1:
@@ -222,6 +223,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
             raise ValueError("nothing to do: norm=False and no table")
         if f32 is not None:
             raise ValueError("norm weights need norm=True")
+    eps, norm, interleaved = float(eps), bool(norm), bool(interleaved)
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     R = 0
@@ -329,7 +331,7 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
         raise ValueError(f"{Hq} query heads cannot share {Hkv} key heads (at most 128 each)")
     if D % 8 or not 8 <= D <= MAX_HEAD_DIM:
         raise ValueError(f"head_dim must be a multiple of 8 up to {MAX_HEAD_DIM}, got {D}")
-    scale = D**-0.5 if scale is None else float(scale)
+    causal, scale = bool(causal), D**-0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite, got {scale}")
     batch = 1

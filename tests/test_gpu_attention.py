@@ -900,3 +900,19 @@ def test_one_module_for_all_blocks_of_a_pass():
         kept = [t.clone() for t in args]
         assert torch.equal(call(*args), blocks(*args))
         assert all(torch.equal(a, b) for a, b in zip(args, kept))
+
+
+def test_numbers_of_numpy_are_numbers():
+    """In the compiled form, in the interpreted one and for outputs that are given alike."""
+    import numpy as np
+
+    q, k, v = qkv(5, 9, 2, 2, 64, seed=102)
+    table = A.rotary_table(torch.arange(5, device=DEV), (64,), theta=np.float32(500.0))
+    assert torch.equal(table, A.rotary_table(torch.arange(5, device=DEV), (64,), theta=500.0))
+    want = A.attention(q, k, v, causal=True, scale=0.25)
+    for kw in ({}, {"out": torch.empty_like(q)}):
+        assert torch.equal(A.attention(q, k, v, causal=np.True_, scale=np.float32(0.25), **kw), want)
+    want = A.qk_norm_rope(q, table=table, eps=0.5, interleaved=False)
+    for kw in ({}, {"q_out": torch.empty_like(q)}):
+        got = A.qk_norm_rope(q, table=table, eps=np.float32(0.5), norm=np.True_, interleaved=np.False_, **kw)
+        assert torch.equal(got, want)
