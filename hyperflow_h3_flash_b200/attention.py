@@ -244,22 +244,21 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
     if q.is_cuda and (Hq == 0 or (k is not None and k_shape[1] == 0)):
         raise ValueError("q and k need at least one head")
     qo, ko = _output(q_out, q, "q_out"), None if k is None else _output(k_out, k, "k_out")
-    if k is not None and not (q_out is None and k_out is None) and qo.numel() and ko.numel():
-        at = qo.data_ptr()
-        if at == k.data_ptr() or at == ko.data_ptr() or ko.data_ptr() == q.data_ptr():
-            raise ValueError("q_out and k_out must not be the other's input or each other")
+    if q.is_cuda or q_out is not None or k_out is not None:
+        qos, q_ptr, qo_ptr = qo.stride(), q.data_ptr(), qo.data_ptr()
+        kk = (None, 0, 0, None, 0, 0, 0)
+        if k is not None:
+            kos, k_ptr, ko_ptr = ko.stride(), k.data_ptr(), ko.data_ptr()
+            if (qo_ptr == k_ptr or qo_ptr == ko_ptr or ko_ptr == q_ptr) and qo.numel() and ko.numel():
+                raise ValueError("q_out and k_out must not be the other's input or each other")
+            kk = (k_ptr, ks[0], ks[1], ko_ptr, kos[0], kos[1], k_shape[1])
     if not q.is_cuda:
         qo.copy_(_norm_rope_torch(q, q_weight, eps, norm, table, interleaved))
         if k is None:
             return qo
         return qo, ko.copy_(_norm_rope_torch(k, k_weight, eps, norm, table, interleaved))
-    qos = qo.stride()
-    kk = (None, 0, 0, None, 0, 0, 0)
-    if k is not None:
-        kos = ko.stride()
-        kk = (k.data_ptr(), ks[0], ks[1], ko.data_ptr(), kos[0], kos[1], k_shape[1])
-    rc = _call(_lib.lib().convrot_qk_norm_rope, q.device, q.data_ptr(), qs[0], qs[1], qo.data_ptr(), qos[0], qos[1], Hq,
-               *kk, T, D, _DTYPES[q.dtype], norm, None if q_weight is None else q_weight.data_ptr(),
+    rc = _call(_lib.lib().convrot_qk_norm_rope, q.device, q_ptr, qs[0], qs[1], qo_ptr, qos[0], qos[1], Hq, *kk, T, D,
+               _DTYPES[q.dtype], norm, None if q_weight is None else q_weight.data_ptr(),
                None if k_weight is None else k_weight.data_ptr(), f32 is True, eps,
                None if table is None else table.data_ptr(), R // 2, R, interleaved)
     if rc:
