@@ -198,8 +198,8 @@ def qk_norm_rope(q: Tensor, k: Tensor | None = None, *, q_weight: Tensor | None 
     (``rotary_table``'s, fp32 ``[T, R / 2, 2]``; None: no rotation): pairs of neighbours if ``interleaved``, else
     ``(j, j + R / 2)``.  fp32 arithmetic, one rounding.  Returns the new q (and k when given).  ``q_out`` / ``k_out`` may
     be the inputs themselves; an output that overlaps an input in any other way is not supported."""
-    if q_out is None and k_out is None and q.is_cuda and (fast := _fast_calls()) is not None:
-        made = fast.qk_norm_rope(q, k, q_weight, k_weight, eps, norm, table, interleaved)
+    if q.is_cuda and (fast := _fast_calls()) is not None:
+        made = fast.qk_norm_rope(q, k, q_weight, k_weight, eps, norm, table, interleaved, q_out, k_out)
         if made is not None:
             return made
     _no_grad(q, k, q_weight, k_weight, table, q_out, k_out)

@@ -76,10 +76,30 @@ bool truth(PyObject* o, int* v) {
   return true;
 }
 
-// qk_norm_rope(q, k, q_weight, k_weight, eps, norm, table, interleaved)
+// The tensor to write into: a given output (null if it needs a second look: an inference tensor has no version to count
+// the write in), else a fresh one, which `made` then holds.
+const at::Tensor* target(PyObject* given, const at::Tensor& like, int device, int type, at::Tensor* made) {
+  if (given == Py_None) {
+    *made = fresh(like);
+    return made;
+  }
+  const at::Tensor* t = heads(given, device, type);
+  return t && t->sizes() == like.sizes() && !t->is_inference() ? t : nullptr;
+}
+
+// An output as the call returns it; the write into a given one counts as torch's own in-place operations do.
+PyObject* returned(PyObject* given, at::Tensor& made) {
+  if (given == Py_None) return THPVariable_Wrap(std::move(made));
+  THPVariable_Unpack(given).unsafeGetTensorImpl()->bump_version();
+  Py_INCREF(given);
+  return given;
+}
+
+// qk_norm_rope(q, k, q_weight, k_weight, eps, norm, table, interleaved[, q_out, k_out])
 PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (!g_rope || n != 8) return nullptr;
+    if (!g_rope || (n != 8 && n != 10)) return nullptr;
+    PyObject* const given[2] = {n == 10 ? a[8] : Py_None, n == 10 ? a[9] : Py_None};
     const int device = c10::cuda::current_device();
     const at::Tensor* q = heads(a[0], device, -1);
     if (!q) return nullptr;
@@ -112,19 +132,26 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return nullptr;
     }
     const int64_t pairs = table ? table->size(1) : 0;
-    at::Tensor qo = fresh(*q), ko;
-    if (k) ko = fresh(*k);
-    const int rc = g_rope(q->data_ptr(), q->stride(0), q->stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
+    if (!k && given[1] != Py_None) return nullptr;
+    at::Tensor made[2];
+    const at::Tensor* qo = target(given[0], *q, device, type, &made[0]);
+    const at::Tensor* ko = k ? target(given[1], *k, device, type, &made[1]) : nullptr;
+    if (!qo || (k && !ko)) return nullptr;
+    if (k && T > 0) {
+      const void *x = qo->data_ptr(), *y = ko->data_ptr();
+      if (x == k->data_ptr() || x == y || y == q->data_ptr()) return nullptr;
+    }
+    const int rc = g_rope(q->data_ptr(), q->stride(0), q->stride(1), qo->data_ptr(), qo->stride(0), qo->stride(1),
                           static_cast<int>(q->size(1)), k ? k->data_ptr() : nullptr, k ? k->stride(0) : 0,
-                          k ? k->stride(1) : 0, k ? ko.data_ptr() : nullptr, k ? ko.stride(0) : 0,
-                          k ? ko.stride(1) : 0, k ? static_cast<int>(k->size(1)) : 0, T, static_cast<int>(D), type,
+                          k ? k->stride(1) : 0, k ? ko->data_ptr() : nullptr, k ? ko->stride(0) : 0,
+                          k ? ko->stride(1) : 0, k ? static_cast<int>(k->size(1)) : 0, T, static_cast<int>(D), type,
                           norm, weight[0], weight[1], f32 == 1, static_cast<float>(eps),
                           table ? static_cast<const float*>(table->data_ptr()) : nullptr, pairs,
                           static_cast<int>(2 * pairs), interleaved, stream_of(device));
     if (rc) return nullptr;
-    if (!k) return THPVariable_Wrap(std::move(qo));
-    PyObject* x = THPVariable_Wrap(std::move(qo));
-    PyObject* y = THPVariable_Wrap(std::move(ko));
+    if (!k) return returned(given[0], made[0]);
+    PyObject* x = returned(given[0], made[0]);
+    PyObject* y = returned(given[1], made[1]);
     PyObject* r = x && y ? PyTuple_Pack(2, x, y) : nullptr;
     Py_XDECREF(x);
     Py_XDECREF(y);

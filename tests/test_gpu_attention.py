@@ -916,3 +916,32 @@ def test_numbers_of_numpy_are_numbers():
     for kw in ({}, {"q_out": torch.empty_like(q)}):
         got = A.qk_norm_rope(q, table=table, eps=np.float32(0.5), norm=np.True_, interleaved=np.False_, **kw)
         assert torch.equal(got, want)
+
+
+def test_compiled_and_interpreted_calls_agree_on_given_outputs():
+    fast = A._fast_calls()
+    q, k, _ = qkv(40, 40, 4, 2, 64, seed=103)
+    table = A.rotary_table(torch.arange(40, device=DEV), (64,))
+    want = A.qk_norm_rope(q, k, table=table)
+    qo, ko = torch.empty(4, 40, 64, dtype=q.dtype, device=DEV).transpose(0, 1), torch.empty_like(k)
+    versions = qo._version, ko._version
+    base = (None, None, 1e-6, True, table, True)
+    for outs in ((qo, ko), (None, ko), (qo, None)):
+        got = fast.qk_norm_rope(q, k, *base, *outs)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(b is None or a is b for a, b in zip(got, outs))
+    assert (qo._version, ko._version) == (versions[0] + 2, versions[1] + 2)
+    assert fast.qk_norm_rope(q, None, *base, qo, None) is qo and torch.equal(qo, want[0])
+    with torch.inference_mode():
+        kept = torch.empty_like(q)
+    for args in ((q, k, *base, k, None), (q, k, *base, None, q), (q, k, *base, qo, qo), (q, q, *base, q, q), (q, None, *base, None, ko),
+                 (q, k, *base, qo[:3], ko), (q, k, *base, qo.half(), ko), (q, k, *base, qo.cpu(), ko), (q, k, *base, kept, ko),
+                 (q, k, *base, qo.clone().requires_grad_(), ko), (q, k, *base, qo)):
+        assert fast.qk_norm_rope(*args) is None
+    inplace = q.clone(), k.clone()
+    back = A.qk_norm_rope(*inplace, table=table, q_out=inplace[0], k_out=inplace[1])
+    assert back[0] is inplace[0] and back[1] is inplace[1] and all(torch.equal(a, b) for a, b in zip(back, want))
+    # (a truth value that is no bool takes the interpreted way)
+    assert fast.qk_norm_rope(q, k, None, None, 1e-6, True, table, 1, None, None) is None
+    for outs in ({}, {"q_out": qo, "k_out": ko}):
+        assert all(torch.equal(a, b) for a, b in zip(A.qk_norm_rope(q, k, table=table, interleaved=1, **outs), want))
