@@ -316,8 +316,8 @@ def attention(q: Tensor, k: Tensor, v: Tensor, *, cu_q: Tensor | None = None, cu
     ``out`` must not overlap the inputs, nor its rows each other.  Scores, statistics and sums are fp32; the weights are
     rounded to the inputs' type for their product with v.  Few queries over long keys are split over the GPU and joined
     in a fixed order: results do not vary from run to run."""
-    if out is None and q.is_cuda and (fast := _fast_calls()) is not None:
-        made = fast.attention(q, k, v, cu_q, cu_k, causal, scale, return_lse)
+    if q.is_cuda and (fast := _fast_calls()) is not None:
+        made = fast.attention(q, k, v, cu_q, cu_k, causal, scale, return_lse, out)
         if made is not None:
             return made
     _no_grad(q, k, v, out)

@@ -159,10 +159,11 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// attention(q, k, v, cu_q, cu_k, causal, scale, return_lse)
+// attention(q, k, v, cu_q, cu_k, causal, scale, return_lse[, out])
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (!g_attention || !g_workspace || n != 8) return nullptr;
+    if (!g_attention || !g_workspace || (n != 8 && n != 9)) return nullptr;
+    PyObject* const given = n == 9 ? a[8] : Py_None;
     const int device = c10::cuda::current_device();
     const at::Tensor* q = heads(a[0], device, -1);
     if (!q) return nullptr;
@@ -191,18 +192,24 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int hq = static_cast<int>(q->size(1)), hkv = static_cast<int>(k->size(1));
     const int64_t size = g_workspace(Tq, Tk, batch, hq, hkv, static_cast<int>(D));
     if (size < 0) return nullptr;
-    at::Tensor out = fresh(*q), lse, space;
+    at::Tensor made, lse, space;
+    const at::Tensor* out = target(given, *q, device, type, &made);
+    if (!out) return nullptr;
+    if (Tq > 0) {
+      const void* o = out->data_ptr();
+      if (o == q->data_ptr() || o == k->data_ptr() || o == v->data_ptr()) return nullptr;
+    }
     if (return_lse) lse = at::empty({Tq, hq}, q->options().dtype(at::kFloat));
     if (size) space = at::empty({size}, q->options().dtype(at::kByte));
     const int rc = g_attention(q->data_ptr(), q->stride(0), q->stride(1), k->data_ptr(), k->stride(0), k->stride(1),
                                v->data_ptr(), v->stride(0), v->stride(1), cu[0], cu[1], batch, Tq, Tk, hq, hkv,
-                               static_cast<int>(D), type, static_cast<float>(scale), causal, out.data_ptr(),
-                               out.stride(0), out.stride(1),
+                               static_cast<int>(D), type, static_cast<float>(scale), causal, out->data_ptr(),
+                               out->stride(0), out->stride(1),
                                return_lse ? static_cast<float*>(lse.data_ptr()) : nullptr,
                                size ? space.data_ptr() : nullptr, static_cast<size_t>(size), stream_of(device));
     if (rc) return nullptr;
-    if (!return_lse) return THPVariable_Wrap(std::move(out));
-    PyObject* x = THPVariable_Wrap(std::move(out));
+    if (!return_lse) return returned(given, made);
+    PyObject* x = returned(given, made);
     PyObject* y = THPVariable_Wrap(std::move(lse));
     PyObject* r = x && y ? PyTuple_Pack(2, x, y) : nullptr;
     Py_XDECREF(x);

@@ -945,3 +945,28 @@ def test_compiled_and_interpreted_calls_agree_on_given_outputs():
     assert fast.qk_norm_rope(q, k, None, None, 1e-6, True, table, 1, None, None) is None
     for outs in ({}, {"q_out": qo, "k_out": ko}):
         assert all(torch.equal(a, b) for a, b in zip(A.qk_norm_rope(q, k, table=table, interleaved=1, **outs), want))
+
+
+def test_compiled_and_interpreted_attention_agree_on_a_given_output():
+    fast = A._fast_calls()
+    q, k, v = qkv(40, 70, 4, 2, 64, seed=104)
+    want, want_lse = A.attention(q, k, v, causal=1, return_lse=True)  # (no bool: the interpreted way)
+    out = torch.empty(4, 40, 64, dtype=q.dtype, device=DEV).transpose(0, 1)
+    version, base = out._version, (None, None, True, None)
+    assert fast.attention(q, k, v, *base, False, out) is out and torch.equal(out, want) and out._version == version + 1
+    out.zero_()
+    got, lse = fast.attention(q, k, v, *base, True, out)
+    assert got is out and torch.equal(out, want) and torch.equal(lse, want_lse)
+    assert A.attention(q, k, v, causal=1, out=out.zero_()) is out and torch.equal(out, want)
+    with torch.inference_mode():
+        kept = torch.empty_like(q)
+    same = q[:, :2].clone()
+    for args in ((q, k, v, *base, False, q), (q, k, v, *base, False, out[:3]), (q, k, v, *base, False, out.half()),
+                 (q, k, v, *base, False, out.cpu()), (q, k, v, *base, False, kept), (same, same, v[:40], *base, False, same),
+                 (q[:, :2], k[:40], v[:40], *base, False, v[:40]), (q, k, v, *base, False, out.clone().requires_grad_())):
+        assert fast.attention(*args) is None
+    # the workspace of a divided call, and rows of no sequence
+    q, k, v = qkv(9, 5000, 4, 2, 64, seed=105)
+    out = torch.full_like(q, 7.0)
+    assert A.attention(q, k, v, cu_q=_cu([1, 3]), cu_k=_cu([4000, 1000]), out=out) is out
+    assert (out[4:] == 7).all() and torch.equal(out[:4], A.attention(q, k, v, cu_q=_cu([1, 3]), cu_k=_cu([4000, 1000]))[:4])
