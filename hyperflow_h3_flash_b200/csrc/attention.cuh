@@ -24,10 +24,10 @@
 // the special-function unit (2^15 exponentials at 16 a cycle); it takes about 3100, since the weights of a tile depend
 // on its scores and the next scores go where the weights were: the two tiles cover each other's latency only in part.
 // ncu on 8192 tokens x 18 heads: tensor pipe 67 % of active cycles, special-function unit 67 %.  32760 tokens x 5
-// heads: 1.94 ms, 1415 TFLOP/s (causal 1.03 ms, 1330) in a burst; 1220 over seconds, where the 1000 W limit brings the
-// clock to 1.5 GHz.  Single tokens over long caches: 5.3 TB/s of keys and values.  Short keys (333) pay 6000 to 8000
-// cycles an item for its first tile, its output and the cold code of both, beside 9500 of steps: 272 us for 32760 x 40
-// heads.
+// heads: 1.95 ms, 1410 TFLOP/s (causal 1.04 ms, 1320) in a burst; 1220 over seconds, where the 1000 W limit brings the
+// clock to 1.5 GHz.  Single tokens over long caches: 5.7 TB/s of keys and values.  Short keys (333) pay 6000 to 8000
+// cycles an item for its first tile, its output and the cold code of both, beside 9500 of steps: 283 us for 32760 x 40
+// heads.  At 64 channels the exponentials alone are the floor: 8192 tokens x 40 heads 0.93 ms of 0.58.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -165,7 +165,8 @@ int64_t attn_items(int64_t Tq, int64_t batch, int heads_q, int heads_kv) {
 //     not; beyond 24 waves the difference is within 1 % either way.
 // The offsets of several sequences are not known here: any of them may be the long one, and may come last.  A sequence of
 // eight times the mean is reckoned with, and CTAs that would idle all the while.  Single tokens, 8 heads, divided / not:
-// 147 requests of 128 keys 26 / 10.6 us, 16 of 2000 keys 39.7 / 28.4, one of 32768 behind 63 of 100 keys 81 / 272.
+// 147 requests of 128 keys 26.1 / 10.6 us, 16 of 2000 keys (40 / 8 heads) 38.9 / 28.6, one of 32768 behind 63 of 100 keys
+// 54.3 / 272.
 int attn_shares(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int D, int sms) {
   // (the sum of at most kMaxShares items' work has to fit an int)
   if (batch < 1 || Tq < 1 || Tk < 8 * kAtTile || Tk > (1 << 28)) return 0;

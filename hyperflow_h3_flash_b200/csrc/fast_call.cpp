@@ -1,8 +1,8 @@
 // The common calls of the attention operators without the interpreter in between (module hyperflow_h3_flash_b200._fast).
 //
 // Each function looks at its arguments as attention.py does and, where nothing about them needs a second look (CUDA
-// tensors on the current device, no gradient wanted, sizes that the library takes), allocates the outputs, calls the C
-// entry on torch's current stream and returns the result.  In every other case it returns None, and attention.py goes
+// tensors on the current device, no gradient wanted, sizes that the library takes), takes the given outputs or allocates
+// them, calls the C entry on torch's current stream and returns the result.  In every other case it returns None, and attention.py goes
 // through its own checks and names what is wrong: nothing is decided here alone.  At a few tokens the checks and the
 // foreign-function call take three times as long as the launch (17 us against 6 for the norm and rotation of 17 tokens).
 #include <ATen/ATen.h>

@@ -187,8 +187,8 @@ int convrot_silu(const void* x, void* y, int64_t n, void* stream);
 /*
  * What an attention block computes between its q / k / v and out projections (no counterpart in the reference, where it
  * is diffusers' code; call sites transformer.py:350-358).  16-bit tensors [T, H, D] are given by a base and their token
- * and head strides in elements (multiples of 8; D contiguous; bases 16-byte aligned), so they may be slices of a wider
- * projection.  dtype: CONVROT_BF16 or CONVROT_FP16 for every 16-bit tensor of a call.
+ * and head strides in elements (positive multiples of 8; D contiguous; bases 16-byte aligned), so they may be slices of
+ * a wider projection.  dtype: CONVROT_BF16 or CONVROT_FP16 for every 16-bit tensor of a call.
  *
  * convrot_rotary_table   the table of a rotation with `axes` position axes (at most 8; time, height, width for video):
  *                        out[t, j] = (cos, sin) of positions[t, a] * theta[a]^(-2 i / dims[a]), fp32 [rows, R / 2, 2],
@@ -205,7 +205,8 @@ int convrot_silu(const void* x, void* y, int64_t n, void* stream);
  * convrot_attention      out = softmax(scale q k^T + mask) v for `batch` sequences packed behind each other: sequence b
  *                        is rows [cu_q[b], cu_q[b + 1]) of q and out and [cu_k[b], cu_k[b + 1]) of k and v (device
  *                        arrays of batch + 1 non-decreasing offsets; both NULL: one sequence, batch 1).  Rows of no
- *                        sequence stay as they were.  Query head h reads key head h / (heads_q / heads_kv).  causal:
+ *                        sequence stay as they were; rows of k and v that are not filled yet can be a sequence without
+ *                        a query.  Query head h reads key head h / (heads_q / heads_kv).  causal:
  *                        query i of lq sees keys up to i + lk - lq.  A row that sees no key gives zeros (lse
  *                        -infinity).  What a row does not see never reaches it, NaN and infinities included.  lse:
  *                        fp32 [Tq, heads_q] natural log-sum-exp, or NULL.  fp32 scores, statistics and sums; softmax
@@ -333,7 +334,10 @@ int convrot_last_cuda_error(void);
  */
 int convrot_poll_error(void* stream);
 
-/* Bounded-wait limit of the GEMM kernels, in nanoseconds of %globaltimer (default 2e9). */
+/*
+ * Limit of the device-side waits, in nanoseconds of %globaltimer (default 2e9; 0 restores it).  In the attention kernel it
+ * counts from the last key or value tile that a block asked for: an item may take longer.
+ */
 void convrot_set_wait_limit_ns(uint64_t ns);
 
 /*
