@@ -156,37 +156,46 @@ int64_t attn_items(int64_t Tq, int64_t batch, int heads_q, int heads_kv) {
 //
 // Dividing saves the time that CTAs without a last item would idle, an item's work times their share, and costs a second
 // launch, a later start of the next kernel and the partial rows' way through memory.  In half steps (one 128 x 128 tile,
-// about 0.8 us of a CTA) the fixed part measured 14 and each megabyte of partial rows about one:
-//   1 token, 8 heads, 1536 / 2048 / 4096 keys (saves 11 / 15 / 30, costs 14): 21.0 / 17.9 / 18.6 us divided, 16.2 / 19.5 /
-//     32.7 not;
-//   256 tokens, 40 heads, 2048 / 4096 / 8192 keys (23 / 47 / 93, 39): 34.0 / 44.4 / 62.4 divided, 32.2 / 58.3 / 109.6 not;
-//   700 tokens, 40 heads, 1024 / 8192 keys, 120 items for 148 CTAs (3 / 24, 49): 48.9 / 157.5 divided, 21.4 / 140.0 not;
-//   4.3 waves of 40 heads, 2048 / 4096 / 32760 keys (22 / 43 / 346, 40): 173.9 / 310.9 / 2236 divided, 165.7 / 320.2 / 2453
+// about 0.8 us of a CTA) the fixed part measured 14 and each megabyte of partial rows 0.8:
+//   1 token, 8 heads, 1536 / 2048 / 4096 keys (saves 11 / 15 / 30, costs 14): 20.7 / 17.6 / 18.4 us divided, 15.8 / 19.0 /
+//     31.8 not;
+//   256 tokens, 40 heads, 2048 / 3000 / 8192 keys (23 / 35 / 93, 34): 33.7 / 39.4 / 61.1 divided, 31.6 / 45.4 / 107.0 not;
+//   4.3 waves of 40 heads, 2048 / 4096 / 32760 keys (22 / 43 / 346, 35): 173.9 / 310.9 / 2236 divided, 165.7 / 320.2 / 2453
 //     not; beyond 24 waves the difference is within 1 % either way.
-// The offsets of several sequences are not known here: any of them may be the long one, and may come last.  A sequence of
-// eight times the mean is reckoned with, and CTAs that would idle all the while.  Single tokens, 8 heads, divided / not:
-// 147 requests of 128 keys 26.1 / 10.6 us, 16 of 2000 keys (40 / 8 heads) 38.9 / 28.6, one of 32768 behind 63 of 100 keys
-// 54.3 / 272.
+// Where less than a fifth of the CTAs would idle, the others slow down by as much (power, L2): 120 items for 148 CTAs over
+// 8192 / 32760 keys 151 / 487 us divided, 133 / 462 not.
+//
+// Of several sequences only the sums of the lengths are known here.  One is reckoned with that has a fourth of all keys or
+// eight times the mean, and eight times the mean queries: its items have the GPU to themselves at last.  If they fill it,
+// half a wave of items of the mean is.  Single tokens, 8 key heads, divided / not: 100 requests of 40 keys 19.7 / 10.3 us
+// (not divided), 16 of 2000 keys 38.9 / 28.6 and 63 of 100 keys before one of 8000 40.7 / 74.4 (divided).  4 prompts of 1000
+// tokens, 8 heads 51.8 / 22.1 (not divided).
 int attn_shares(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int D, int sms) {
   // (the sum of at most kMaxShares items' work has to fit an int)
   if (batch < 1 || Tq < 1 || Tk < 8 * kAtTile || Tk > (1 << 28)) return 0;
   const int shares = sms < kMaxShares ? sms : kMaxShares, group = heads_q / heads_kv;
   const int64_t items = attn_items(Tq, batch, heads_q, heads_kv);
   if (items >= 24 * static_cast<int64_t>(shares)) return 0;
-  auto longest = [&](int64_t all) {
-    const int64_t eightfold = 8 * ((all + batch - 1) / batch);
-    return eightfold < all ? eightfold : all;
-  };
-  const int64_t last = batch == 1 ? items % shares : items < shares ? items : shares - 1;
+  auto at_most = [](int64_t a, int64_t b) { return a < b ? a : b; };
+  const int64_t tile = kAtTile / group;  // query positions
+  int64_t queries = (Tq + batch - 1) / batch, keys = (Tk + batch - 1) / batch, last = items % shares, idle = shares - last;
+  const int64_t long_queries = at_most(Tq, 8 * queries);
+  const int64_t long_items = (long_queries + 2 * tile - 1) / (2 * tile) * heads_kv;
+  if (batch > 1 && long_items < shares) {
+    queries = long_queries;
+    keys = at_most(Tk, 8 * keys > Tk / 4 ? 8 * keys : Tk / 4);
+    last = at_most(items, shares - 1);
+    idle = shares - long_items;
+  } else if (batch > 1) {
+    last = idle = shares / 2;
+  }
   // (one sequence whose items fill whole waves: nothing is left to divide and nothing is launched for it, unless offsets
   // make it shorter)
-  if (last == 0) return shares;
-  const int64_t rows = longest(Tq) * group, tile_rows = kAtTile / group * group;
-  const int64_t units = (longest(Tk) + kAtTile - 1) / kAtTile * (rows > tile_rows ? 2 : 1);
-  const int64_t idle = batch == 1 ? shares - last : shares;
-  const int64_t cuts = units * last / 8 < shares ? units * last / 8 : shares;
-  const int64_t part_bytes = (cuts + last) * (rows < 2 * tile_rows ? rows : 2 * tile_rows) * D * 4;
-  return units * idle > (14 + part_bytes / 1000000) * shares ? shares : 0;
+  if (batch == 1 && last == 0) return shares;
+  const int64_t units = (keys + kAtTile - 1) / kAtTile * (queries > tile ? 2 : 1);
+  const int64_t parts = at_most(units * last / 8, shares) + last;
+  const int64_t part_bytes = parts * at_most(queries, 2 * tile) * group * D * 4;
+  return 5 * idle >= shares && units * idle > (14 + part_bytes / 1250000) * shares ? shares : 0;
 }
 
 size_t attn_workspace(int shares, int D) {

@@ -654,10 +654,10 @@ NO_PLAN = [  # shares, items, first item, all work, then the work before each it
 def test_a_plan_that_was_never_written_leads_nowhere(plan, causal):
     """Offsets of sequences that overlap, which the arrays must not hold, make more items than the grid has CTAs, and
     the plan for the joining kernel is not written: whatever the workspace held, nothing outside the outputs is."""
-    T, heads = 4096, 20
+    T, heads = 8192, 2
     q, k, v = qkv(T, T, heads, heads, 64, seed=80)
-    cu = torch.tensor([0, T] * 4, dtype=torch.int32, device=DEV)
-    size = _lib.lib().convrot_attention_workspace_size(T, T, 7, heads, heads, 64)
+    cu = torch.tensor([0, T] * 10, dtype=torch.int32, device=DEV)
+    size = _lib.lib().convrot_attention_workspace_size(T, T, 19, heads, heads, 64)
     assert size > 0
     space = torch.zeros(size // 4, dtype=torch.int32, device=DEV)
     space[:4] = torch.tensor(plan[:4])
@@ -766,9 +766,9 @@ def test_a_last_wave_that_is_divided_behind_whole_ones(D):
     assert size(2560, 8192, 1, 20, 20, D) > 0
     check(q, k, v, [2560], [8192], cu=False)
     check(q, k, v, [2560], [8192], True, cu=False)
-    lq, lk = [300, 1, 2000, 0, 259], [100, 5000, 2000, 13, 1079]
-    assert size(2560, 8192, 5, 20, 20, D) > 0
-    check(q, k, v, lq, lk, True)
+    lq, lk = [1200, 1, 1359], [6000, 8013, 2371]
+    assert size(2560, 16384, 3, 20, 20, D) > 0
+    check(q, torch.cat([k, k]), torch.cat([v, v]), lq, lk, True)
 
 
 def test_which_calls_are_divided():
@@ -777,10 +777,11 @@ def test_which_calls_are_divided():
     if torch.cuda.get_device_properties(0).multi_processor_count != 148:
         pytest.skip("the sizes are for 148 SMs")
     for Tq, Tk, batch, hq, hkv, divided in (
-            (1, 1536, 1, 8, 8, False), (1, 2048, 1, 8, 8, True), (256, 2048, 1, 40, 40, False), (256, 4096, 1, 40, 40, True),
-            (700, 1024, 1, 40, 40, False), (700, 8192, 1, 40, 40, False), (4096, 2048, 1, 40, 40, False),
+            (1, 1536, 1, 8, 8, False), (1, 2048, 1, 8, 8, True), (256, 2048, 1, 40, 40, False), (256, 3000, 1, 40, 40, True),
+            (700, 1024, 1, 40, 40, False), (700, 32760, 1, 40, 40, False), (4096, 2048, 1, 40, 40, False),
             (4096, 4096, 1, 40, 40, True), (32760, 32760, 1, 5, 5, True), (32760, 333, 1, 40, 40, False),
-            (147, 147 * 128, 147, 8, 1, False), (64, 63 * 100 + 32768, 64, 40, 8, True), (17, 333, 1, 8, 8, False)):
+            (33093, 33093, 2, 5, 5, True), (100, 4000, 100, 8, 1, False), (64, 63 * 100 + 8000, 64, 40, 8, True),
+            (4000, 4000, 4, 8, 8, False), (8720, 8720, 4, 40, 40, False), (1024, 8300, 4, 8, 8, True), (17, 333, 1, 8, 8, False)):
         assert (size(Tq, Tk, batch, hq, hkv, 128) > 0) == divided, (Tq, Tk, batch, hq, hkv)
 
 
