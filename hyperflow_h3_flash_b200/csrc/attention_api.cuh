@@ -166,10 +166,12 @@ int64_t attn_items(int64_t Tq, int64_t batch, int heads_q, int heads_kv) {
 // 8192 / 32760 keys 151 / 487 us divided, 133 / 462 not.
 //
 // Of several sequences only the sums of the lengths are known here.  One is reckoned with that has a fourth of all keys or
-// eight times the mean, and eight times the mean queries: its items have the GPU to themselves at last.  If they fill it,
-// half a wave of items of the mean is.  Single tokens, 8 key heads, divided / not: 100 requests of 40 keys 19.7 / 10.3 us
-// (not divided), 16 of 2000 keys 38.9 / 28.6 and 63 of 100 keys before one of 8000 40.7 / 74.4 (divided).  4 prompts of 1000
-// tokens, 8 heads 51.8 / 22.1 (not divided).
+// eight times the mean, and eight times the mean queries too unless the keys are twice the queries (chunks and tokens behind
+// caches): its items have the GPU to themselves at last.  If they fill it, half a wave of items of the mean is reckoned
+// with.  Single tokens, 8 key heads, divided / not: 100 requests of 40 keys 19.7 / 10.3 us (not divided), 16 of 2000 keys
+// 38.9 / 28.6 and 63 of 100 keys before one of 8000 40.3 / 74.7 (divided).  4 prompts of 1000 tokens, 8 heads 51.8 / 21.8
+// (not divided).  Chunks of 256 queries, 40 heads, 15 over 200 keys before one over 16000 137 / 247, 40 over 2000 keys 526 /
+// 479 (divided).
 int attn_shares(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv, int D, int sms) {
   // (the sum of at most kMaxShares items' work has to fit an int)
   if (batch < 1 || Tq < 1 || Tk < 8 * kAtTile || Tk > (1 << 28)) return 0;
@@ -179,7 +181,7 @@ int attn_shares(int64_t Tq, int64_t Tk, int64_t batch, int heads_q, int heads_kv
   auto at_most = [](int64_t a, int64_t b) { return a < b ? a : b; };
   const int64_t tile = kAtTile / group;  // query positions
   int64_t queries = (Tq + batch - 1) / batch, keys = (Tk + batch - 1) / batch, last = items % shares, idle = shares - last;
-  const int64_t long_queries = at_most(Tq, 8 * queries);
+  const int64_t long_queries = Tk / 2 >= Tq ? queries : at_most(Tq, 8 * queries);
   const int64_t long_items = (long_queries + 2 * tile - 1) / (2 * tile) * heads_kv;
   if (batch > 1 && long_items < shares) {
     queries = long_queries;

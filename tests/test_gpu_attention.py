@@ -781,7 +781,8 @@ def test_which_calls_are_divided():
             (700, 1024, 1, 40, 40, False), (700, 32760, 1, 40, 40, False), (4096, 2048, 1, 40, 40, False),
             (4096, 4096, 1, 40, 40, True), (32760, 32760, 1, 5, 5, True), (32760, 333, 1, 40, 40, False),
             (33093, 33093, 2, 5, 5, True), (100, 4000, 100, 8, 1, False), (64, 63 * 100 + 8000, 64, 40, 8, True),
-            (4000, 4000, 4, 8, 8, False), (8720, 8720, 4, 40, 40, False), (1024, 8300, 4, 8, 8, True), (17, 333, 1, 8, 8, False)):
+            (4000, 4000, 4, 8, 8, False), (8720, 8720, 4, 40, 40, False), (1024, 8300, 4, 8, 8, True),
+            (40 * 256, 39 * 200 + 32768, 40, 40, 40, True), (40 * 256, 40 * 500, 40, 40, 40, False), (17, 333, 1, 8, 8, False)):
         assert (size(Tq, Tk, batch, hq, hkv, 128) > 0) == divided, (Tq, Tk, batch, hq, hkv)
 
 
